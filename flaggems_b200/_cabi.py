@@ -46,6 +46,13 @@ _SIGS = {
     "fg_silu_and_mul": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
     "fg_moe_sum": (c_int, [_P, _P, c_int64, c_int, c_int64, c_int, _P]),
     "fg_moe_sum_indexed": (c_int, [_P, _P, c_int64, c_int, c_int64, c_int, _P, _P, _P]),
+    "fg_moe_permute": (
+        c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, _P, c_int, c_int64, c_int, c_int, c_int64, c_int, c_int64, c_int64,
+                c_int64, _P]),
+    "fg_moe_unpermute": (
+        c_int, [_P, _P, _P, _P, c_int, c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
+    "fg_moe_unpermute_backward": (
+        c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
     "fg_gather_rows_fp8": (
         c_int, [_P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int32, c_int32, _P, _P]),
     "fg_moe_align_block_size_ex": (
@@ -77,6 +84,9 @@ _SIGS = {
     "fg_scaled_grouped_mm_fp8": (
         c_int, [_P, _P, _P, _P, _P, _P, c_int64, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int,
                 _P, c_int64, _P]),
+    "fg_scaled_grouped_mm_int8": (
+        c_int, [_P, _P, _P, _P, _P, _P, c_int64, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int,
+                _P, c_int64, _P]),
     "fg_group_ids_from_offsets": (c_int, [_P, c_int, c_int64, _P, _P]),
     "fg_grouped_gemm_fp8_bias": (
         c_int, [_P, _P, _P, _P, _P, _P, c_int64, _P, _P, _P, c_int64, c_int64, c_int, c_int64, c_int64, c_int64,
@@ -87,6 +97,9 @@ _SIGS = {
     "fg_symm_free": (c_int, [_P]),
     "fg_scaled_mm_fp8": (
         c_int, [_P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                c_int, c_int, c_int, c_int, _P]),
+    "fg_scaled_mm_int8": (
+        c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                 c_int, c_int, c_int, c_int, _P]),
     "fg_block_scaled_mm_fp8": (
         c_int, [_P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,

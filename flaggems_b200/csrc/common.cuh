@@ -80,9 +80,17 @@ struct FgGroupedGemm {
 };
 int fg_grouped_gemm(const FgGroupedGemm& g, cudaStream_t stream);
 
+// The rows of a grouped product's result that follow its last group, to be filled with zeros (c NULL: left as they are).
+struct FgTail {
+    void* c;
+    int64_t ld;  // elements
+    int64_t n;
+    int elem_size;
+};
+
 // sorted_ids / expert_ids / num_post_pad of rows grouped by the ends `offs`, padded to `block` per group.
 int fg_group_tiles(const int32_t* offs, int num_groups, int64_t rows, int block, int32_t* sorted_ids, int64_t max_pad,
-                   int32_t* expert_ids, int64_t n_blocks, int32_t* num_post_pad, cudaStream_t stream);
+                   int32_t* expert_ids, int64_t n_blocks, int32_t* num_post_pad, const FgTail& tail, cudaStream_t stream);
 
 // fg_moe_align_block_size_regions; fill_tail = false leaves the entries past the last block unwritten.
 int fg_moe_align(const void* topk_ids, int ids_are_i64, int64_t numel, int num_experts, int block_size, const int32_t* expert_map,

@@ -293,8 +293,8 @@ __device__ __forceinline__ TileCoord tile_coord(int t, int num_m, int num_n) {
 // distributed shared memory (no global scratch, no atomics).  For decode-sized M, where there are
 // fewer tiles than SMs and the job is to pull the weights from HBM with every SM.
 // OPK (operand kind): 0 = e4m3 (kind::f8f6f4); 1 = signed 8-bit integers with 32-bit integer accumulators
-// (kind::i8) for the int8 w8a8 expert GEMMs (the epilogue converts the accumulators to fp32 and applies
-// the per-row x per-column scales); 2 / 3 = bf16 / f16 (kind::f16) for the unquantised and
+// (kind::i8) for the int8 w8a8 products, dense and grouped (the epilogue converts the accumulators to fp32 and
+// applies the per-row x per-column scales; split-K adds the integers, so any split gives the same bits); 2 / 3 = bf16 / f16 (kind::f16) for the unquantised and
 // weight-only-quantised expert GEMMs.  The main loop is written in bytes (a K block is 128 bytes of a
 // K-major row, an MMA consumes 32 of them), so a 16-bit product of K elements runs as 2K bytes.
 template <int BN, bool BLOCK_SCALED, bool FUSE_SILU, bool SMALL_A, bool SPLITK, bool PAIR = false, bool ASTORE = false,
@@ -305,7 +305,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     using C = Cfg<BN, SMALL_A, PAIR, ASTORE, !BLOCK_SCALED && !SPLITK>;
     static_assert(!ASTORE || (BLOCK_SCALED && !SPLITK), "the store warp serves the block-scaled tiles");
     constexpr bool INT8 = OPK == 1;
-    static_assert(OPK == 0 || (!BLOCK_SCALED && !SPLITK && !SMALL_A), "int8 and 16-bit operands serve the plain and grouped tiles");
+    static_assert(OPK == 0 || !BLOCK_SCALED, "block scales are for e4m3 operands");
+    static_assert(OPK < 2 || (!SPLITK && !SMALL_A), "16-bit operands serve the grouped tiles");
     // accumulator word -> fp32
     auto acc_f = [](uint32_t raw) -> float {
         if constexpr (INT8) return __int2float_rn((int)raw);
@@ -1125,12 +1126,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             const int n_epi = C::EPI_WARPS * 32;
             for (int idx = threadIdx.x - C::FIRST_EPI_WARP * 32; idx < rows * vec_per_row; idx += n_epi) {
                 const int r = idx / vec_per_row, c = c_first + (idx % vec_per_row) * 4;
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                using Part = std::conditional_t<INT8, int4, float4>;
+                Part sum{};
                 for (int q = 0; q < k_slices; ++q) {
-                    const float4 v = *reinterpret_cast<const float4*>(part[q] + (size_t)r * (BN + 4) + c);
+                    const Part v = *reinterpret_cast<const Part*>(part[q] + (size_t)r * (BN + 4) + c);
                     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
                 }
-                float o[4] = {sum.x, sum.y, sum.z, sum.w};
+                float o[4] = {(float)sum.x, (float)sum.y, (float)sum.z, (float)sum.w};
                 const int64_t row = (int64_t)m0 + r;
                 if constexpr (!BLOCK_SCALED) {
                     const float sa = p.sa_mode == FG_SCALE_VECTOR ? p.sa[row] : p.sa[0];
@@ -1209,7 +1211,7 @@ int make_map(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_
 }
 
 // How many clusters of `slices` CTAs of the split-K kernel fit on the device at once (cached).
-template <int BN, bool BS>
+template <int BN, bool BS, int OPK = 0>
 int max_resident_clusters(int slices) {
     static int table[64][9];
     static std::mutex mu;
@@ -1217,7 +1219,7 @@ int max_resident_clusters(int slices) {
     int* cache = table[fg_device_index()];
     if (cache[slices]) return cache[slices];
     using C = Cfg<BN, false>;
-    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true>;
+    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true, false, false, OPK>;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(slices * 64), 1, 1);
@@ -1239,11 +1241,11 @@ int max_resident_clusters(int slices) {
     return n;
 }
 
-template <int BN, bool BS>
+template <int BN, bool BS, int OPK = 0>
 int launch_splitk(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, int tiles, int slices,
                   cudaStream_t st) {
     using C = Cfg<BN, false>;
-    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true>;
+    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true, false, false, OPK>;
     static bool attr_done[64];
     static std::mutex mu;
     {
@@ -1375,7 +1377,9 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
         const int64_t nkb = fg_cdiv(p.K, BLOCK_K);
         for (int cand = 8; cand >= 2; cand /= 2) {
             const int64_t per = fg_cdiv(nkb, cand);
-            const int resident = wide == 256
+            const int resident = p.int8 == 1
+                ? (wide == 256 ? max_resident_clusters<256, false, 1>(cand) : max_resident_clusters<128, false, 1>(cand))
+                : wide == 256
                 ? (block_scaled ? max_resident_clusters<256, true>(cand) : max_resident_clusters<256, false>(cand))
                 : (block_scaled ? max_resident_clusters<128, true>(cand) : max_resident_clusters<128, false>(cand));
             if (wide_tiles <= resident && per >= 2 && (cand - 1) * per < nkb) {
@@ -1422,8 +1426,15 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
 
     const int t = (int)tiles;
     if (p.int8) {
-        FG_REQUIRE(!block_scaled && (bn == 256 || bn == 128) && k_slices == 1 && !pair, FG_ERR_UNSUPPORTED,
-                   "int8 and 16-bit operands are built for the grouped expert GEMMs");
+        FG_REQUIRE(!block_scaled && (p.int8 == 1 || p.grouped), FG_ERR_UNSUPPORTED,
+                   "int8 operands take no block scales, and 16-bit operands are built for the grouped expert GEMMs");
+        if (!p.grouped) {
+            if (k_slices > 1) return bn == 256 ? launch_splitk<256, false, 1>(ta, tb, p, t, k_slices, st)
+                                               : launch_splitk<128, false, 1>(ta, tb, p, t, k_slices, st);
+            if (bn == 64) return launch_inst<64, false, false, false, false, 1>(ta, tb, p, t, st);
+            if (small_a) return launch_inst<32, false, false, true, false, 1>(ta, tb, p, t, st);
+            if (bn == 32) return launch_inst<32, false, false, false, false, 1>(ta, tb, p, t, st);
+        }
         auto by_kind = [&](auto bn_tag, auto silu_tag) -> int {
             constexpr int B = decltype(bn_tag)::value;
             constexpr bool S = decltype(silu_tag)::value;
@@ -1486,6 +1497,29 @@ __global__ void bounded_wait_selftest_kernel(unsigned int* status, uint64_t limi
     }
 }
 
+// Dense product of e4m3 (operand 0) or int8 (1) operands.
+int scaled_mm_common(int operand, void* c, const void* a, const void* b, const float* sa, const float* sb, const void* bias,
+                     int bias_dtype, int64_t M, int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c, int sa_mode,
+                     int sb_mode, int out_dtype, int bias_after_round, void* stream) {
+    FG_REQUIRE(M >= 0 && N >= 0 && K >= 0, FG_ERR_INVALID_ARGUMENT, "negative size");
+    if (M == 0 || N == 0) return FG_OK;
+    FG_REQUIRE(c && a && b && sa && sb, FG_ERR_INVALID_ARGUMENT, "null pointer");
+    FG_REQUIRE(dtype_ok(out_dtype) || (operand == 0 && out_dtype == FG_DTYPE_E4M3), FG_ERR_INVALID_ARGUMENT, "bad out_dtype %d", out_dtype);
+    FG_REQUIRE((sa_mode == FG_SCALE_SCALAR || sa_mode == FG_SCALE_VECTOR) &&
+                   (sb_mode == FG_SCALE_SCALAR || sb_mode == FG_SCALE_VECTOR),
+               FG_ERR_INVALID_ARGUMENT, "scale modes must be scalar or vector");
+    FG_REQUIRE(N < (1ll << 31) && K < (1ll << 31) && M < (1ll << 31), FG_ERR_UNSUPPORTED, "dimension too large");
+    GemmParams p{};
+    p.M = M; p.N = (int)N; p.K = (int)K; p.n_out = (int)N;
+    p.c = c; p.ld_c = ld_c; p.out_dtype = out_dtype;
+    p.sa = sa; p.sb = sb; p.bias = bias; p.sa_mode = sa_mode; p.sb_mode = sb_mode;
+    p.bias_after_round = bias_after_round;
+    p.bias_dtype = bias_dtype;
+    p.block_rows = BLOCK_M;
+    p.int8 = operand;
+    return launch_gemm(p, a, M, ld_a, b, 1, ld_b, false, false, (cudaStream_t)stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1512,23 +1546,21 @@ int fg_selftest_bounded_wait(int64_t limit_ns, int site, void* stream) {
 int fg_scaled_mm_fp8(void* c, const void* a, const void* b, const float* sa, const float* sb, const void* bias,
                      int64_t M, int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c, int sa_mode,
                      int sb_mode, int out_dtype, int bias_after_round, void* stream) {
-    FG_REQUIRE(M >= 0 && N >= 0 && K >= 0, FG_ERR_INVALID_ARGUMENT, "negative size");
-    if (M == 0 || N == 0) return FG_OK;
-    FG_REQUIRE(c && a && b && sa && sb, FG_ERR_INVALID_ARGUMENT, "null pointer");
-    FG_REQUIRE(dtype_ok(out_dtype) || out_dtype == FG_DTYPE_E4M3, FG_ERR_INVALID_ARGUMENT, "bad out_dtype %d", out_dtype);
-    FG_REQUIRE((sa_mode == FG_SCALE_SCALAR || sa_mode == FG_SCALE_VECTOR) &&
-                   (sb_mode == FG_SCALE_SCALAR || sb_mode == FG_SCALE_VECTOR),
-               FG_ERR_INVALID_ARGUMENT, "scale modes must be scalar or vector");
-    FG_REQUIRE(N < (1ll << 31) && K < (1ll << 31) && M < (1ll << 31), FG_ERR_UNSUPPORTED, "dimension too large");
-    GemmParams p{};
-    p.M = M; p.N = (int)N; p.K = (int)K; p.n_out = (int)N;
-    p.c = c; p.ld_c = ld_c; p.out_dtype = out_dtype;
-    p.sa = sa; p.sb = sb; p.bias = bias; p.sa_mode = sa_mode; p.sb_mode = sb_mode;
-    p.bias_after_round = bias_after_round;
-    p.bias_dtype = out_dtype == FG_DTYPE_E4M3 ? FG_DTYPE_F32 : out_dtype;  // fp32 bias only with the e4m3 output
-    p.block_rows = BLOCK_M;
-    return launch_gemm(p, a, M, ld_a, b, 1, ld_b, false, false, (cudaStream_t)stream);
+    // fp32 bias only with the e4m3 output
+    return scaled_mm_common(0, c, a, b, sa, sb, bias, out_dtype == FG_DTYPE_E4M3 ? FG_DTYPE_F32 : out_dtype, M, N, K, ld_a, ld_b,
+                            ld_c, sa_mode, sb_mode, out_dtype, bias_after_round, stream);
 }
+
+int fg_scaled_mm_int8(void* c, const void* a, const void* b, const float* sa, const float* sb, const void* bias,
+                      int bias_dtype, int64_t M, int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c,
+                      int sa_mode, int sb_mode, int out_dtype, int bias_after_round, void* stream) {
+    FG_REQUIRE(!bias || dtype_ok(bias_dtype), FG_ERR_INVALID_ARGUMENT, "bad bias_dtype %d", bias_dtype);
+    FG_REQUIRE(K <= FG_INT8_MAX_K, FG_ERR_UNSUPPORTED, "K = %lld: sums of more than %d int8 products may leave 32 bits",
+               (long long)K, FG_INT8_MAX_K);
+    return scaled_mm_common(1, c, a, b, sa, sb, bias, bias_dtype, M, N, K, ld_a, ld_b, ld_c, sa_mode, sb_mode, out_dtype,
+                            bias_after_round, stream);
+}
+
 
 int fg_block_scaled_mm_fp8(void* c, const void* a, const void* b, const float* a_s, const float* b_s, int64_t M,
                            int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c, int64_t ld_as,

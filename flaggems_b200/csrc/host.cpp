@@ -210,8 +210,8 @@ PyObject* act_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// token_quant(x) -> (q, s): one scale per row
-PyObject* token_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// token_quant(x) -> (q, s) and token_quant_int8(x): one scale per row
+PyObject* token_quant_as(ScalarType to, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         int64_t m, k, ld;
         const at::Tensor* x = n == 1 ? cuda_tensor(a[0]) : nullptr;
@@ -219,15 +219,18 @@ PyObject* token_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor q, s;
         const int rc = unlocked([&] {
             c10::cuda::CUDAGuard guard(x->device());
-            q = empty(x->sizes(), E4M3, *x);
+            q = empty(x->sizes(), to, *x);
             s = empty(sizes_with_last(*x, 1), ScalarType::Float, *x);
-            return fg_per_token_quant_fp8(x->data_ptr(), dtype_code(x->scalar_type()), q.data_ptr(),
-                                          static_cast<float*>(s.data_ptr()), m, k, ld, k, nullptr, 1, 0, nullptr, stream_of(*x));
+            auto entry = to == E4M3 ? fg_per_token_quant_fp8 : fg_per_token_quant_int8;
+            return entry(x->data_ptr(), dtype_code(x->scalar_type()), q.data_ptr(), static_cast<float*>(s.data_ptr()), m, k, ld,
+                         k, nullptr, 1, 0, nullptr, stream_of(*x));
         });
         if (rc != FG_OK) return raise_rc(rc);
         return pair(std::move(q), std::move(s));
     });
 }
+PyObject* token_quant(PyObject*, PyObject* const* a, Py_ssize_t n) { return token_quant_as(E4M3, a, n); }
+PyObject* token_quant_int8(PyObject*, PyObject* const* a, Py_ssize_t n) { return token_quant_as(ScalarType::Char, a, n); }
 
 // tensor_quant(x, scale) -> q: the given scale for the whole tensor
 PyObject* tensor_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -307,14 +310,16 @@ PyObject* scaled_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
         if (n != 7) return none();
         const at::Tensor *c = cuda_tensor(p[0]), *a = cuda_tensor(p[1]), *b = cuda_tensor(p[2]), *sa = cuda_tensor(p[3]),
                          *sb = cuda_tensor(p[4]);
-        if (!c || !a || !b || !sa || !sb || a->scalar_type() != E4M3 || b->scalar_type() != E4M3) return none();
+        const bool cutlass = p[6] == Py_True;
+        if (!c || !a || !b || !sa || !sb || a->scalar_type() != b->scalar_type()) return none();
+        const bool int8 = cutlass && a->scalar_type() == ScalarType::Char;  // aten _scaled_mm has no int8 operands
+        if (!int8 && a->scalar_type() != E4M3) return none();
         if (a->dim() != 2 || b->dim() != 2 || c->dim() != 2) return none();
         const int64_t m = a->size(0), k = a->size(1), cols = b->size(1);
         const int code = c->scalar_type() == E4M3 ? FG_DTYPE_E4M3 : dtype_code(c->scalar_type());
         if (code < 0 || m == 0 || cols == 0 || b->size(0) != k || c->size(0) != m || c->size(1) != cols) return none();
         if (a->stride(1) != 1 || a->stride(0) % 16 || c->stride(1) != 1 || !k_contiguous(*b)) return none();
         if (!scale_ok(*sa, m) || !scale_ok(*sb, cols)) return none();
-        const bool cutlass = p[6] == Py_True;
         if (cutlass) {
             if (c->stride(0) % 16 || code == FG_DTYPE_E4M3) return none();
         } else {
@@ -329,6 +334,12 @@ PyObject* scaled_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
         }
         const int rc = unlocked([&] {
             c10::cuda::CUDAGuard guard(a->device());
+            if (int8)
+                return fg_scaled_mm_int8(c->data_ptr(), a->data_ptr(), b->data_ptr(), static_cast<const float*>(sa->data_ptr()),
+                                         static_cast<const float*>(sb->data_ptr()), bias ? bias->data_ptr() : nullptr, code, m,
+                                         cols, k, a->stride(0), b->stride(1), c->stride(0),
+                                         sa->numel() > 1 ? FG_SCALE_VECTOR : FG_SCALE_SCALAR,
+                                         sb->numel() > 1 ? FG_SCALE_VECTOR : FG_SCALE_SCALAR, code, 1, stream_of(*a));
             return fg_scaled_mm_fp8(c->data_ptr(), a->data_ptr(), b->data_ptr(), static_cast<const float*>(sa->data_ptr()),
                                     static_cast<const float*>(sb->data_ptr()), bias ? bias->data_ptr() : nullptr, m, cols, k,
                                     a->stride(0), b->stride(1), c->stride(0), sa->numel() > 1 ? FG_SCALE_VECTOR : FG_SCALE_SCALAR,
@@ -353,6 +364,86 @@ PyObject* scaled_mm_new(PyObject* self, PyObject* const* p, Py_ssize_t n) {
         PyObject* r = scaled_mm(self, args, 7);
         Py_DECREF(c);
         return r;
+    });
+}
+
+// int8_mm(A, B, As, Bs, bias or None, output dtype) -> C: A [..., K] and B [N, K] int8
+PyObject* int8_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        ScalarType out;
+        int64_t m, k, ld;
+        if (n != 6 || !py_dtype(p[5], &out) || dtype_code(out) < 0) return none();
+        const at::Tensor *a = cuda_tensor(p[0]), *b = cuda_tensor(p[1]), *sa = cuda_tensor(p[2]), *sb = cuda_tensor(p[3]);
+        if (!a || !b || !sa || !sb || a->scalar_type() != ScalarType::Char || b->scalar_type() != ScalarType::Char) return none();
+        if (a->device() != b->device() || a->device() != sa->device() || a->device() != sb->device()) return none();
+        if (!as_rows(*a, &m, &k, &ld) || ld % 16 || ld < k || (uintptr_t)a->data_ptr() % 16 || b->dim() != 2 || b->size(1) != k)
+            return none();
+        const int64_t cols = b->size(0);
+        if (cols == 0 || b->stride(1) != 1 || b->stride(0) % 16 || b->stride(0) < k || (uintptr_t)b->data_ptr() % 16) return none();
+        if (!scale_ok(*sa, m) || !scale_ok(*sb, cols)) return none();
+        // one value per row: the shape of the rows, with or without a last 1
+        if (sa->numel() > 1) {
+            const auto lead = a->sizes().slice(0, a->dim() - 1);
+            const bool last = sa->dim() == a->dim() && sa->size(-1) == 1;
+            if (!(sa->dim() + 1 == a->dim() && sa->sizes() == lead) && !(last && sa->sizes().slice(0, lead.size()) == lead)) return none();
+        }
+        if (sb->numel() > 1 && !(sb->dim() == 1 || (sb->dim() == 2 && sb->size(1) == 1))) return none();
+        const at::Tensor* bias = nullptr;
+        if (p[4] != Py_None) {
+            bias = cuda_tensor(p[4]);
+            if (!bias || dtype_code(bias->scalar_type()) < 0 || bias->dim() != 1 || bias->size(0) != cols || !bias->is_contiguous() ||
+                bias->device() != a->device())
+                return none();
+        }
+        at::Tensor c;
+        const int rc = unlocked([&] {
+            c10::cuda::CUDAGuard guard(a->device());
+            c = empty(sizes_with_last(*a, cols), out, *a);
+            return fg_scaled_mm_int8(c.data_ptr(), a->data_ptr(), b->data_ptr(), static_cast<const float*>(sa->data_ptr()),
+                                     static_cast<const float*>(sb->data_ptr()), bias ? bias->data_ptr() : nullptr,
+                                     bias ? dtype_code(bias->scalar_type()) : 0, m, cols, k, ld, b->stride(0), cols,
+                                     sa->numel() > 1 ? FG_SCALE_VECTOR : FG_SCALE_SCALAR,
+                                     sb->numel() > 1 ? FG_SCALE_VECTOR : FG_SCALE_SCALAR, dtype_code(out), 0, stream_of(*a));
+        });
+        if (rc != FG_OK) return raise_rc(rc);
+        return THPVariable_Wrap(std::move(c));
+    });
+}
+
+// int8_grouped_mm(A, B, As, Bs, offs, output dtype) -> C: rows of A [M, K] grouped by offs, B [G, N, K], both int8
+PyObject* int8_grouped_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        ScalarType out;
+        if (n != 6 || !py_dtype(p[5], &out) || dtype_code(out) < 0) return none();
+        const at::Tensor *a = cuda_tensor(p[0]), *b = cuda_tensor(p[1]), *sa = cuda_tensor(p[2]), *sb = cuda_tensor(p[3]),
+                         *offs = cuda_tensor(p[4]);
+        if (!a || !b || !sa || !sb || !offs || a->scalar_type() != ScalarType::Char || b->scalar_type() != ScalarType::Char) return none();
+        for (const at::Tensor* t : {b, sa, sb, offs})
+            if (t->device() != a->device()) return none();
+        if (a->dim() != 2 || b->dim() != 3 || sb->dim() != 2 || offs->dim() != 1) return none();
+        const int64_t m = a->size(0), k = a->size(1), groups = b->size(0), cols = b->size(1);
+        if (m == 0 || cols == 0 || groups == 0 || k == 0 || k % 16 || b->size(2) != k || !b->is_contiguous()) return none();
+        if (a->stride(1) != 1 || a->stride(0) % 16 || a->stride(0) < k || (uintptr_t)a->data_ptr() % 16 ||
+            (uintptr_t)b->data_ptr() % 16)
+            return none();
+        if (sa->scalar_type() != ScalarType::Float || sa->numel() != m || !sa->is_contiguous() ||
+            !(sa->dim() == 1 || (sa->dim() == 2 && sa->size(1) == 1)) || sb->scalar_type() != ScalarType::Float ||
+            sb->size(0) != groups || sb->size(1) != cols || !sb->is_contiguous() || offs->scalar_type() != ScalarType::Int ||
+            offs->size(0) != groups || !offs->is_contiguous())
+            return none();
+        at::Tensor c, ws;
+        const int rc = unlocked([&] {
+            c10::cuda::CUDAGuard guard(a->device());
+            c = empty({m, cols}, out, *a);
+            const int64_t need = fg_scaled_grouped_mm_workspace_bytes(m, (int)groups, k) + 256;
+            ws = empty({need}, ScalarType::Byte, *a);
+            return fg_scaled_grouped_mm_int8(c.data_ptr(), a->data_ptr(), b->data_ptr(), static_cast<const float*>(sa->data_ptr()),
+                                             static_cast<const float*>(sb->data_ptr()), nullptr, 0,
+                                             static_cast<const int32_t*>(offs->data_ptr()), (int)groups, m, cols, k, a->stride(0),
+                                             cols, dtype_code(out), ws.data_ptr(), need, stream_of(*a));
+        });
+        if (rc != FG_OK) return raise_rc(rc);
+        return THPVariable_Wrap(std::move(c));
     });
 }
 
@@ -582,6 +673,7 @@ PyObject* fused_experts(PyObject*, PyObject* const* p, Py_ssize_t n) {
 PyMethodDef methods[] = {
     FG_METHOD(group_quant), FG_METHOD(act_quant),    FG_METHOD(token_quant), FG_METHOD(tensor_quant),
     FG_METHOD(block_mm),    FG_METHOD(scaled_mm),    FG_METHOD(scaled_mm_new), FG_METHOD(grouped_mm),
+    FG_METHOD(token_quant_int8), FG_METHOD(int8_mm), FG_METHOD(int8_grouped_mm),
     FG_METHOD(topk_softmax), FG_METHOD(grouped_topk), FG_METHOD(moe_align),  FG_METHOD(silu_mul),
     FG_METHOD(moe_sum),     FG_METHOD(fused_experts), {nullptr, nullptr, 0, nullptr}};
 

@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(256) group_ids_kernel(const int32_t* offs, int
 __global__ void __launch_bounds__(ALIGN_THREADS, 1) group_tiles_kernel(const int32_t* offs, int num_groups,
                                                                        int32_t rows, int32_t block, int32_t* sorted_ids,
                                                                        int64_t max_pad, int32_t* expert_ids,
-                                                                       int64_t n_blocks, int32_t* num_post_pad) {
+                                                                       int64_t n_blocks, int32_t* num_post_pad, FgTail tail) {
     fg_pdl_wait();
     fg_pdl_trigger();
     __shared__ int32_t first[ALIGN_THREADS], pad_first[ALIGN_THREADS + 1], scan_tmp[ALIGN_WARPS];
@@ -437,6 +437,18 @@ __global__ void __launch_bounds__(ALIGN_THREADS, 1) group_tiles_kernel(const int
         sorted_ids[p] = id;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) num_post_pad[0] = total;
+    if (tail.c) {
+        const int64_t end = min(max(offs[num_groups - 1], 0), rows), bytes = tail.n * tail.elem_size, ld = tail.ld * tail.elem_size;
+        const bool vec = ((reinterpret_cast<uintptr_t>(tail.c) | (uintptr_t)ld | (uintptr_t)bytes) & 15) == 0;
+        for (int64_t r = end + blockIdx.x; r < rows; r += gridDim.x) {
+            uint8_t* row = reinterpret_cast<uint8_t*>(tail.c) + r * ld;
+            if (vec) {
+                for (int64_t b = threadIdx.x * 16; b < bytes; b += ALIGN_THREADS * 16) *reinterpret_cast<uint4*>(row + b) = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+                for (int64_t b = threadIdx.x * 2; b < bytes; b += ALIGN_THREADS * 2) *reinterpret_cast<uint16_t*>(row + b) = 0;
+            }
+        }
+    }
 }
 
 __global__ void __launch_bounds__(256) fill_ones_kernel(float* x, int64_t n) {
@@ -556,11 +568,11 @@ int fg_fill_ones(float* x, int64_t n, cudaStream_t stream) {
 }
 
 int fg_group_tiles(const int32_t* offs, int num_groups, int64_t rows, int block, int32_t* sorted_ids, int64_t max_pad,
-                   int32_t* expert_ids, int64_t n_blocks, int32_t* num_post_pad, cudaStream_t stream) {
+                   int32_t* expert_ids, int64_t n_blocks, int32_t* num_post_pad, const FgTail& tail, cudaStream_t stream) {
     FG_REQUIRE(num_groups > 0 && num_groups <= ALIGN_THREADS && block > 0, FG_ERR_UNSUPPORTED, "at most %d groups", ALIGN_THREADS);
     FG_REQUIRE(rows + (int64_t)num_groups * block < (1ll << 31), FG_ERR_UNSUPPORTED, "too many rows");
     const int64_t blocks = fg_cdiv(max_pad, ALIGN_THREADS);
-    FG_CUDA(fg_launch(group_tiles_kernel, (unsigned)(blocks < fg_num_sms() ? blocks : fg_num_sms()), ALIGN_THREADS, 0, stream, 1, offs, num_groups, (int32_t)rows, block, sorted_ids, max_pad, expert_ids, n_blocks, num_post_pad));
+    FG_CUDA(fg_launch(group_tiles_kernel, (unsigned)(blocks < fg_num_sms() ? blocks : fg_num_sms()), ALIGN_THREADS, 0, stream, 1, offs, num_groups, (int32_t)rows, block, sorted_ids, max_pad, expert_ids, n_blocks, num_post_pad, tail));
     return FG_OK;
 }
 

@@ -241,6 +241,38 @@ Workspace carve_grouped_mm(void* base, int64_t m_total, int num_groups, int tile
     return w;
 }
 
+// aten _scaled_grouped_mm on e4m3 (operand 0) or its counterpart on int8 operands (1).
+int scaled_grouped_mm(int operand, void* c, const void* a, const void* b, const float* scale_a, const float* scale_b,
+                      const float* bias, int64_t bias_stride_g, const int32_t* offs, int num_groups,
+                      int64_t m_total, int64_t N, int64_t K, int64_t ld_a, int64_t ld_c, int out_dtype,
+                      void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+    FG_REQUIRE(m_total >= 0 && N > 0 && K > 0 && num_groups > 0, FG_ERR_INVALID_ARGUMENT, "bad sizes");
+    FG_REQUIRE(num_groups <= 1024, FG_ERR_UNSUPPORTED, "at most 1024 groups");
+    FG_REQUIRE(K % 16 == 0, FG_ERR_UNSUPPORTED, "K = %lld must be a multiple of 16", (long long)K);
+    if (m_total == 0) return FG_OK;
+    FG_REQUIRE(c && a && b && scale_a && scale_b && offs && workspace, FG_ERR_INVALID_ARGUMENT, "null pointer");
+    FG_REQUIRE((uintptr_t)workspace % 256 == 0, FG_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    FG_REQUIRE(ld_a % 16 == 0 && (uintptr_t)a % 16 == 0, FG_ERR_UNSUPPORTED, "a must have 16-byte aligned rows");
+    const bool pairs = use_pairs(m_total, num_groups, N, N);
+    const int tile = pairs ? PAIR_ROWS : TILE_ROWS;
+    const Workspace ws = carve_grouped_mm(workspace, m_total, num_groups, tile);
+    FG_REQUIRE(workspace_bytes >= ws.bytes, FG_ERR_INVALID_ARGUMENT, "workspace holds %lld bytes, needs %lld",
+               (long long)workspace_bytes, (long long)ws.bytes);
+    // int8: the rows past the last group become zeros
+    const FgTail tail{operand == 1 ? c : nullptr, ld_c, N, out_dtype == FG_DTYPE_F32 ? 4 : 2};
+    int rc = fg_group_tiles(offs, num_groups, m_total, tile, ws.sorted_ids, ws.max_pad, ws.expert_ids, ws.n_blocks,
+                            ws.post_pad, tail, st);
+    if (rc != FG_OK) return rc;
+    FgGroupedGemm g{};
+    g.operand = operand;
+    g.sorted_ids = ws.sorted_ids; g.expert_ids = ws.expert_ids; g.num_post_pad = ws.post_pad; g.max_rows = ws.rows;
+    g.numel = m_total; g.num_experts = num_groups; g.block_rows = tile; g.cta_pairs = pairs; g.scale_mode = FG_SCALE_VECTOR; g.out_dtype = out_dtype;
+    g.c = c; g.a = a; g.w = b; g.a_scale = scale_a; g.w_scale = scale_b; g.bias = bias; g.bias_stride = bias_stride_g;
+    // few rows per group: only they are fetched; otherwise a block is one box from its first row
+    g.a_rows = m_total; g.gather_div = 1; g.a_contiguous = !use_gather(m_total, num_groups); g.N = N; g.K = K; g.ld_a = ld_a; g.ld_c = ld_c; g.scatter = 1;
+    return fg_grouped_gemm(g, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -259,29 +291,18 @@ int fg_scaled_grouped_mm_fp8(void* c, const void* a, const void* b, const float*
                              const float* bias, int64_t bias_stride_g, const int32_t* offs, int num_groups,
                              int64_t m_total, int64_t N, int64_t K, int64_t ld_a, int64_t ld_c, int out_dtype,
                              void* workspace, int64_t workspace_bytes, void* stream) {
-    FG_REQUIRE(m_total >= 0 && N > 0 && K > 0 && num_groups > 0, FG_ERR_INVALID_ARGUMENT, "bad sizes");
-    FG_REQUIRE(num_groups <= 1024, FG_ERR_UNSUPPORTED, "at most 1024 groups");
-    FG_REQUIRE(K % 16 == 0, FG_ERR_UNSUPPORTED, "K = %lld must be a multiple of 16", (long long)K);
-    if (m_total == 0) return FG_OK;
-    FG_REQUIRE(c && a && b && scale_a && scale_b && offs && workspace, FG_ERR_INVALID_ARGUMENT, "null pointer");
-    FG_REQUIRE((uintptr_t)workspace % 256 == 0, FG_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
-    FG_REQUIRE(ld_a % 16 == 0 && (uintptr_t)a % 16 == 0, FG_ERR_UNSUPPORTED, "a must have 16-byte aligned rows");
-    const bool pairs = use_pairs(m_total, num_groups, N, N);
-    const int tile = pairs ? PAIR_ROWS : TILE_ROWS;
-    const Workspace ws = carve_grouped_mm(workspace, m_total, num_groups, tile);
-    FG_REQUIRE(workspace_bytes >= ws.bytes, FG_ERR_INVALID_ARGUMENT, "workspace holds %lld bytes, needs %lld",
-               (long long)workspace_bytes, (long long)ws.bytes);
-    cudaStream_t st = (cudaStream_t)stream;
-    int rc = fg_group_tiles(offs, num_groups, m_total, tile, ws.sorted_ids, ws.max_pad, ws.expert_ids, ws.n_blocks,
-                            ws.post_pad, st);
-    if (rc != FG_OK) return rc;
-    FgGroupedGemm g{};
-    g.sorted_ids = ws.sorted_ids; g.expert_ids = ws.expert_ids; g.num_post_pad = ws.post_pad; g.max_rows = ws.rows;
-    g.numel = m_total; g.num_experts = num_groups; g.block_rows = tile; g.cta_pairs = pairs; g.scale_mode = FG_SCALE_VECTOR; g.out_dtype = out_dtype;
-    g.c = c; g.a = a; g.w = b; g.a_scale = scale_a; g.w_scale = scale_b; g.bias = bias; g.bias_stride = bias_stride_g;
-    // few rows per group: only they are fetched; otherwise a block is one box from its first row
-    g.a_rows = m_total; g.gather_div = 1; g.a_contiguous = !use_gather(m_total, num_groups); g.N = N; g.K = K; g.ld_a = ld_a; g.ld_c = ld_c; g.scatter = 1;
-    return fg_grouped_gemm(g, st);
+    return scaled_grouped_mm(0, c, a, b, scale_a, scale_b, bias, bias_stride_g, offs, num_groups, m_total, N, K, ld_a, ld_c,
+                             out_dtype, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+int fg_scaled_grouped_mm_int8(void* c, const void* a, const void* b, const float* scale_a, const float* scale_b,
+                              const float* bias, int64_t bias_stride_g, const int32_t* offs, int num_groups,
+                              int64_t m_total, int64_t N, int64_t K, int64_t ld_a, int64_t ld_c, int out_dtype,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+    FG_REQUIRE(K <= FG_INT8_MAX_K, FG_ERR_UNSUPPORTED, "K = %lld: sums of more than %d int8 products may leave 32 bits",
+               (long long)K, FG_INT8_MAX_K);
+    return scaled_grouped_mm(1, c, a, b, scale_a, scale_b, bias, bias_stride_g, offs, num_groups, m_total, N, K, ld_a, ld_c,
+                             out_dtype, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 int64_t fg_moe_routed_workspace_bytes(int64_t n_rows_in, int num_experts, int64_t H, int64_t I) {

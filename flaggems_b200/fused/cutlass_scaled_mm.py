@@ -1,9 +1,10 @@
-"""cutlass_scaled_mm: c = (a_scale * b_scale) * (a @ b) [+ bias] for FP8 operands.
+"""cutlass_scaled_mm: c = (a_scale * b_scale) * (a @ b) [+ bias] for FP8 and int8 operands.
 
 Mirrors src/flag_gems/fused/cutlass_scaled_mm.py:475-526 (checks) and :371-431
 (dispatch on the scale shapes) of the reference.  Where the reference raises
 NotImplementedError on compute capability 10.x (:459-460), this runs the tcgen05
-kernels of ``fg_scaled_mm_fp8`` / ``fg_block_scaled_mm_fp8``.
+kernels of ``fg_scaled_mm_fp8`` / ``fg_block_scaled_mm_fp8``, and int8 operands, which the
+reference refuses there (:399-402), those of ``fg_scaled_mm_int8``.
 """
 import logging
 from typing import Optional
@@ -48,10 +49,9 @@ def cutlass_scaled_mm(
 
     m, k = a.shape
     n = b.size(1)
-    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
-        if a.dtype == torch.int8:
-            raise RuntimeError("Int8 not supported on SM100. Use FP8 quantization instead, or run on older arch (SM < 100).")
-        raise AssertionError(f"Unsupported dtype: {a.dtype}")
+    int8 = a.dtype == torch.int8
+    if a.dtype != b.dtype or not (int8 or a.dtype == torch.float8_e4m3fn):
+        raise AssertionError(f"Unsupported dtype: {a.dtype} and {b.dtype}")
     if c.dtype not in _cabi.DTYPE_CODE:
         raise NotImplementedError(f"unsupported output dtype {c.dtype}")
     L = _cabi.lib()
@@ -64,16 +64,18 @@ def cutlass_scaled_mm(
             assert b_scale.is_contiguous(), "b_scale must be contiguous"
             if bias is not None and bias.dtype != c.dtype:
                 bias = bias.to(c.dtype)
+            entry, bias_dtype = (L.fg_scaled_mm_int8, (_cabi.DTYPE_CODE[c.dtype],)) if int8 else (L.fg_scaled_mm_fp8, ())
             _cabi.check(
-                L.fg_scaled_mm_fp8(
+                entry(
                     _cabi.ptr(c), _cabi.ptr(a), _cabi.ptr(b), _cabi.ptr(a_scale), _cabi.ptr(b_scale), _cabi.ptr(bias),
-                    m, n, k, a.stride(0), b.stride(1), c.stride(0),
+                    *bias_dtype, m, n, k, a.stride(0), b.stride(1), c.stride(0),
                     _cabi.SCALE_VECTOR if a_scale.numel() > 1 else _cabi.SCALE_SCALAR,
                     _cabi.SCALE_VECTOR if b_scale.numel() > 1 else _cabi.SCALE_SCALAR,
                     _cabi.DTYPE_CODE[c.dtype], 1, stream,
                 )
             )
         else:
+            assert not int8, "int8 operands take per-tensor or per-token and per-channel scales"
             assert a_scale.dim() == 2, "a_scale must be 2D tensor for blockwise scaling"
             assert b_scale.dim() == 2, "b_scale must be 2D tensor for blockwise scaling"
             assert a.size(0) == a_scale.size(0), (

@@ -20,6 +20,7 @@ from typing import Optional
 import torch
 
 from .. import _cabi
+from ..ops.per_token_quant_int8 import per_token_quant_int8
 from .moe_align_block_size import ceil_div
 
 logger = logging.getLogger(__name__.replace("flaggems_b200", "flag_gems", 1))
@@ -100,9 +101,7 @@ def _int8_quantize(A, A_scale, per_act_token, block_shape=None):
     _cabi.require_cuda(A)
     if block_shape is not None or not per_act_token:
         raise NotImplementedError("int8 activations: only per-token quantisation is implemented")
-    with _cabi.device_guard(A):
-        q, s = _per_token_quant_int8(A)
-    return q.reshape(A.shape), s.reshape(A.shape[:-1] + (1,))
+    return per_token_quant_int8(A)
 
 
 def _group_quant(x, group, row_index=None, index_div=1, index_limit=0, n_rows_dev=None, out_rows=None):
@@ -201,6 +200,8 @@ def moe_kernel_quantize_input(A, A_scale, quant_dtype, per_act_token_quant, bloc
         return A, A_scale
     if quant_dtype == torch.float8_e4m3fn:
         return _fp8_quantize(A, A_scale, per_act_token_quant, block_shape)
+    if quant_dtype == torch.int8:
+        return _int8_quantize(A, A_scale, per_act_token_quant, block_shape)
     raise NotImplementedError(f"quant dtype {quant_dtype} is not implemented")
 
 

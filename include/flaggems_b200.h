@@ -199,6 +199,35 @@ int fg_moe_sum(const void* in, void* out, int64_t M, int topk, int64_t K, int dt
 int fg_moe_sum_indexed(const void* in, void* out, int64_t M, int topk, int64_t K, int dtype,
                        const int32_t* row_index, const void* addend, void* stream);
 
+/* Tokens sorted by expert (no counterpart in the reference, which gathers inside its expert kernel,
+ * src/flag_gems/fused/fused_moe.py:1101-1110).  topk_ids [T, topk]; the expert of a slot is its id, or expert_map[id]
+ * (nullable); slots whose id or mapped id is outside the range have no expert.
+ *   offs[e]               end of expert e's rows (ascending; offs[e - 1] is its begin)
+ *   row_of_slot[t, k]     the slot's row; ~row (negative) for slots without an expert, which come last
+ *   slot_of_row[r]        t * topk + k; rows of an expert are in ascending slot order
+ *   rows[r]               x[t] (elem_bytes 1, 2 or 4 per value, row stride ld_x elements); zeros without an expert
+ *   row_scale[r]          scale[t] (scale_cols values, row stride ld_scale; scale_cols may be 0); ones without an expert
+ * rows and row_scale are contiguous.  At most 1024 experts, T * topk < 2^31 - 1. */
+int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_slot, int32_t* slot_of_row, const void* x,
+                   const float* scale, const void* topk_ids, int ids_are_i64, const int32_t* expert_map, int expert_map_len,
+                   int64_t T, int topk, int num_experts, int64_t H, int elem_bytes, int64_t ld_x, int64_t scale_cols,
+                   int64_t ld_scale, void* stream);
+
+/* out[t] = sum_k weights[t, k] * rows[row_of_slot[t, k]], in fp32 in slot order, rounded once (out [T, H] contiguous, rows
+ * [n_rows, H] of the same dtype).  weights nullable (ones), w_dtype bf16, fp16 or fp32, row stride ld_w.  Slots with a
+ * negative row (or one past n_rows) add nothing and are not read.  With the gradient of fg_moe_permute's rows in
+ * place of rows and no weights this is its backward pass. */
+int fg_moe_unpermute(void* out, const void* rows, const int32_t* row_of_slot, const void* weights, int w_dtype, int64_t T,
+                     int topk, int64_t n_rows, int64_t H, int64_t ld_rows, int64_t ld_w, int dtype, void* stream);
+
+/* The gradients of fg_moe_unpermute, d_rows [n_rows, H] and d_weights [T, topk] of w_dtype, both contiguous and
+ * either of them nullable: d_rows[row] = weights[t, k] * d_out[t], rows of slots without an expert zero;
+ * d_weights[t, k] = <d_out[t], rows[row]> in fp32 in a fixed order, 0 without an expert.  row_of_slot is
+ * fg_moe_permute's, where every row belongs to one slot. */
+int fg_moe_unpermute_backward(void* d_rows, void* d_weights, const void* d_out, const void* rows, const int32_t* row_of_slot,
+                              const void* weights, int w_dtype, int64_t T, int topk, int64_t n_rows, int64_t H, int64_t ld_d_out,
+                              int64_t ld_rows, int64_t ld_w, int dtype, void* stream);
+
 /* Copies FP8 rows [*, K] and their fp32 scale rows [*, s_cols] into a new row order:
  * output row r takes source row row_index[r] / index_div when 0 <= row_index[r] < index_limit,
  * else zeros (scales 1).  The A-operand gather the reference does inside fused_moe_kernel
@@ -367,6 +396,16 @@ int fg_scaled_mm_fp8(void* c, const void* a, const void* b, const float* sa, con
                      int64_t ld_c, int sa_mode, int sb_mode, int out_dtype, int bias_after_round,
                      void* stream);
 
+/* The same product on signed 8-bit operands with 32-bit integer accumulation (tcgen05 kind::i8).  The reference's
+ * cutlass_scaled_mm takes int8 operands on other architectures (src/flag_gems/fused/cutlass_scaled_mm.py:399-402); here
+ * they are taken too.  a int8 [M,K], b int8 [N,K], both K-contiguous with 16-byte aligned rows, K % 16 == 0.  The sums are
+ * whole numbers held exactly, which needs K <= FG_INT8_MAX_K; they are rounded to fp32 once and scaled.
+ * bias (nullable) has bias_dtype; out_dtype bf16, fp16 or fp32. */
+#define FG_INT8_MAX_K 131071 /* 2^14 * K, the largest sum of |products|, stays below 2^31 */
+int fg_scaled_mm_int8(void* c, const void* a, const void* b, const float* sa, const float* sb, const void* bias,
+                      int bias_dtype, int64_t M, int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c,
+                      int sa_mode, int sb_mode, int out_dtype, int bias_after_round, void* stream);
+
 /* w8a8_block_fp8_matmul / fp8_matmul / blockwise cutlass_scaled_mm:
  * src/flag_gems/ops/w8a8_block_fp8_matmul.py:173-232 (kernel :51-122),
  * src/flag_gems/ops/fp8_matmul.py:137-205,
@@ -446,6 +485,13 @@ int fg_scaled_grouped_mm_fp8(void* c, const void* a, const void* b, const float*
                              const float* bias, int64_t bias_stride_g, const int32_t* offs, int num_groups,
                              int64_t m_total, int64_t N, int64_t K, int64_t ld_a, int64_t ld_c, int out_dtype,
                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same on int8 operands (K <= FG_INT8_MAX_K), with the same workspace; rows [offs[-1], m_total) of c become zeros
+ * (fg_scaled_grouped_mm_fp8 leaves them as they are).  No counterpart in the reference. */
+int fg_scaled_grouped_mm_int8(void* c, const void* a, const void* b, const float* scale_a, const float* scale_b,
+                              const float* bias, int64_t bias_stride_g, const int32_t* offs, int num_groups,
+                              int64_t m_total, int64_t N, int64_t K, int64_t ld_a, int64_t ld_c, int out_dtype,
+                              void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Pieces of the above.  fg_group_ids_from_offsets: ids[r] = number of offsets <= r (the group of
  * row r; num_groups for rows past the last end).  fg_grouped_gemm_fp8_bias: the grouped GEMM of

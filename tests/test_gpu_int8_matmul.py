@@ -1,0 +1,296 @@
+"""Products of int8 operands against the definition in 64 bits.
+
+Tolerances count roundings.  The sum of products is a whole number, exact in 32 bits, and is rounded to fp32 once; two scales
+multiply it: three relative errors of 2^-24.  The bias joins with one rounding of the result, the cast adds half a step
+of the output type (fp16 results below its normal range: half of 2^-24).
+"""
+import pytest
+import torch
+
+import flag_gems
+from flaggems_b200 import _cabi
+
+pytestmark = pytest.mark.gpu
+I8 = torch.int8
+F32 = 2.0 ** -24
+
+
+def _ints(g, *shape, lo=-128, hi=128):
+    return torch.randint(lo, hi, shape, generator=g, dtype=I8, device="cuda")
+
+
+def _operands(m, n, k, seed=0, lo=-128):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    a, b = _ints(g, m, k, lo=lo), _ints(g, n, k, lo=lo)
+    a_s = torch.rand(m, 1, device="cuda", generator=g) * 0.02 + 1e-3
+    b_s = torch.rand(n, device="cuda", generator=g) * 0.002 + 1e-4
+    return a, b, a_s, b_s, g
+
+
+def _definition(a, b, a_s, b_s):
+    return (a.double() @ b.double().t()) * a_s.double().reshape(-1, 1) * b_s.double().reshape(1, -1)
+
+
+def _check(got, pre, bias=None, rounded_before_bias=False):
+    """``pre``: the scaled product in 64 bits; ``bias`` joins before the cast, or after it in the output's type."""
+    half = torch.finfo(got.dtype).eps / 2
+    want = pre if bias is None else pre + bias.double()
+    bound = pre.abs() * 3 * F32 + want.abs() * (half + F32 + half * 4 * F32)
+    if rounded_before_bias:
+        bound = bound + pre.abs() * half * (1 + half)
+    if got.dtype == torch.float16:
+        bound = bound + 2.0 ** -25 * (2 if rounded_before_bias else 1)
+    err = (got.double() - want).abs()
+    assert bool((err <= bound * 1.001).all()), (float(err.max()), float((err / bound.clamp_min(1e-300)).max()))
+
+
+# one row block of every tile width, split K, the narrow tiles, ragged edges in every dimension, the CTA pair
+SHAPES = [(1, 1, 16), (1, 256, 128), (1, 6144, 4096), (1, 2112, 7168), (2, 33, 48), (7, 130, 2064), (16, 28672, 4096), (31, 4096, 4096),
+          (32, 300, 16), (33, 208, 496), (64, 24576, 1040), (83, 7744, 3888), (128, 4096, 14336), (129, 144, 144), (130, 4097, 528),
+          (257, 9500, 256), (1024, 6144, 4096), (1037, 6145, 4096), (4099, 8191, 512), (8192, 8192, 1024)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_per_token_per_channel(m, n, k):
+    a, b, a_s, b_s, _ = _operands(m, n, k)
+    _check(flag_gems.w8a8_int8_matmul(a, b, a_s, b_s), _definition(a, b, a_s, b_s))
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 300])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float16, torch.float32])
+def test_types_and_bias(m, out, bias):
+    a, b, a_s, b_s, g = _operands(m, 515, 208, seed=m)
+    c = None if bias is None else torch.randn(515, device="cuda", generator=g).to(bias)
+    got = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, c, out)
+    assert got.dtype == out
+    _check(got, _definition(a, b, a_s, b_s), c)
+
+
+@pytest.mark.parametrize("m", [1, 3, 200])
+def test_scale_shapes(m):
+    a, b, a_s, b_s, _ = _operands(m, 96, 64)
+    one = torch.tensor(0.01, device="cuda")
+    for sa in (a_s, a_s[:, 0], one, one.view(1), one.view(1, 1)):
+        for sb in (b_s, b_s[:, None], one, one.view(1), one.view(1, 1)):
+            _check(flag_gems.w8a8_int8_matmul(a, b, sa, sb), _definition(a, b, sa.reshape(-1), sb.reshape(-1)))
+
+
+def test_more_than_two_dimensions():
+    a, b, a_s, b_s, _ = _operands(30, 72, 48)
+    want = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s)
+    for sa in (a_s.view(5, 6, 1), a_s.view(5, 6)):
+        got = flag_gems.w8a8_int8_matmul(a.view(5, 6, 48), b, sa, b_s)
+        assert got.shape == (5, 6, 72) and torch.equal(got.view(30, 72), want)
+    got = flag_gems.w8a8_int8_matmul(a[0], b, a_s[0], b_s)
+    assert got.shape == (72,) and torch.equal(got, want[0])
+    part = flag_gems.w8a8_int8_matmul(a.view(5, 6, 48).transpose(0, 1), b, a_s.view(5, 6, 1).transpose(0, 1), b_s)
+    assert torch.equal(part.transpose(0, 1).reshape(30, 72), want)
+
+
+def test_strides_and_alignment():
+    a, b, a_s, b_s, g = _operands(37, 80, 64)
+    want = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s)
+    wide_a, wide_b = _ints(g, 37, 160), _ints(g, 80, 160)
+    for off in (0, 16, 1, 7):  # aligned rows of a wider matrix are read where they are, others from a copy
+        wide_a[:, off:off + 64] = a
+        wide_b[:, off:off + 64] = b
+        assert torch.equal(flag_gems.w8a8_int8_matmul(wide_a[:, off:off + 64], wide_b[:, off:off + 64], a_s, b_s), want)
+    assert torch.equal(flag_gems.w8a8_int8_matmul(a.t().contiguous().t(), b.t().contiguous().t(), a_s, b_s), want)
+    row = a[:1]
+    got = flag_gems.w8a8_int8_matmul(row.expand(37, 64), b, a_s, b_s)  # one row for all, stride 0
+    assert torch.equal(got, flag_gems.w8a8_int8_matmul(row.repeat(37, 1), b, a_s, b_s))
+    every_other = torch.empty(160, device="cuda")[::2]
+    every_other.copy_(b_s)
+    assert torch.equal(flag_gems.w8a8_int8_matmul(a, b, a_s, every_other), want)
+
+
+@pytest.mark.parametrize("m", [1, 16, 300])
+def test_sums_at_the_edge_of_32_bits(m):
+    """K as large as it may be with every product 2^14: the largest sum is 2^31 - 2^18."""
+    k = 131056
+    a = torch.full((m, k), -128, dtype=I8, device="cuda")
+    b = torch.full((257, k), -128, dtype=I8, device="cuda")
+    b[1::2] = 127
+    one = torch.ones(1, device="cuda")
+    got = flag_gems.w8a8_int8_matmul(a, b, one, one, None, torch.float32)
+    want = (torch.where(torch.arange(257, device="cuda") % 2 == 0, 128 * 128 * k, -128 * 127 * k)).expand(m, 257)
+    assert torch.equal(got, want.double().float())
+
+
+def test_nothing_to_compute():
+    one = torch.ones(1, device="cuda")
+    a, b = torch.zeros(0, 64, dtype=I8, device="cuda"), torch.zeros(32, 64, dtype=I8, device="cuda")
+    assert flag_gems.w8a8_int8_matmul(a, b, one, one).shape == (0, 32)
+    assert flag_gems.w8a8_int8_matmul(b, a, one, one).shape == (32, 0)
+
+
+def test_special_scales():
+    a, b, a_s, b_s, _ = _operands(40, 64, 64)
+    a_s[3], a_s[5], b_s[7] = float("inf"), float("nan"), 0.0
+    got = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s)
+    want = _definition(a, b, a_s, b_s)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    keep = [i for i in range(40) if i not in (3, 5)]
+    _check(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (33, 208, 496), (700, 4096, 256)])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
+def test_cutlass_scaled_mm(m, n, k, bias, out):
+    a, b, a_s, b_s, g = _operands(m, n, k)
+    c = torch.full((m, n), float("nan"), dtype=out, device="cuda")
+    t = torch.randn(n, device="cuda", generator=g).to(out) if bias else None
+    flag_gems.cutlass_scaled_mm(c, a, b.t(), a_s, b_s, t)
+    _check(c, _definition(a, b, a_s, b_s), t, rounded_before_bias=bias)
+
+
+def test_cutlass_scaled_mm_refusals():
+    a, b, a_s, b_s, _ = _operands(16, 128, 256)
+    c = torch.empty(16, 128, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(AssertionError, match="Unsupported dtype"):
+        flag_gems.cutlass_scaled_mm(c, a, b.to(torch.float8_e4m3fn).t(), a_s, b_s)
+    with pytest.raises(AssertionError, match="int8 operands take"):
+        flag_gems.cutlass_scaled_mm(c, a, b.t(), torch.ones(16, 2, device="cuda"), torch.ones(2, 1, device="cuda"))
+    with pytest.raises(NotImplementedError, match="implemented for float8"):
+        flag_gems.scaled_mm(a, b.t(), a_s, b_s.view(1, -1), None, None, torch.bfloat16)  # aten's op stays an FP8 one
+
+
+# ---- grouped ----------------------------------------------------------------------------------
+def _grouped(sizes, n, k, seed=0, tail=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    m = sum(sizes) + tail
+    a, b = _ints(g, m, k), _ints(g, len(sizes), n, k)
+    a_s = torch.rand(m, 1, device="cuda", generator=g) * 0.02 + 1e-3
+    b_s = torch.rand(len(sizes), n, device="cuda", generator=g) * 0.002 + 1e-4
+    offs = torch.tensor(sizes, device="cuda").cumsum(0).to(torch.int32)
+    return a, b, a_s, b_s, offs, g
+
+
+def _grouped_definition(a, b, a_s, b_s, offs):
+    out = torch.zeros(a.shape[0], b.shape[1], dtype=torch.float64, device="cuda")
+    begin = 0
+    for e, end in enumerate(offs.tolist()):
+        out[begin:end] = _definition(a[begin:end], b[e], a_s[begin:end], b_s[e])
+        begin = end
+    return out
+
+
+SIZES = [[1], [0, 1, 0], [5, 0, 31, 1], [0, 0, 129], [128, 256, 127], [1] * 70, [3, 0, 2, 1, 0, 0, 4] * 20, [800, 900, 1000],
+         [0, 1300], [2000, 1, 0, 700]]
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=[f"{len(s)}x{sum(s)}" for s in SIZES])
+@pytest.mark.parametrize("n,k", [(64, 128), (513, 272), (4096, 64)])
+def test_grouped(sizes, n, k):
+    a, b, a_s, b_s, offs, _ = _grouped(sizes, n, k)
+    _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs), _grouped_definition(a, b, a_s, b_s, offs))
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tail", [1, 200])
+@pytest.mark.parametrize("n", [64, 65])
+def test_grouped_rows_behind_the_last_group_are_zeros(out, tail, n):
+    a, b, a_s, b_s, offs, _ = _grouped([7, 0, 30], n, 64, tail=tail)
+    junk = [torch.full((37 + tail, n), float("nan"), dtype=out, device="cuda") for _ in range(4)]  # memory that is reused
+    del junk
+    got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s[:, 0], b_s, offs, output_dtype=out)
+    _check(got, _grouped_definition(a, b, a_s, b_s, offs))
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert not flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, none, output_dtype=out).any()
+
+
+@pytest.mark.parametrize("per_group", [False, True])
+def test_grouped_bias_strides_and_copies(per_group):
+    a, b, a_s, b_s, offs, g = _grouped([9, 0, 140], 96, 64)
+    bias = torch.randn((3, 96) if per_group else (96,), device="cuda", generator=g)
+    got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs, bias, torch.float32)
+    group = torch.tensor([0] * 9 + [2] * 140, device="cuda")
+    _check(got, _grouped_definition(a, b, a_s, b_s, offs), bias[group] if per_group else bias.expand(149, 96))
+    want = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs)
+    wide = _ints(g, 149, 131)
+    wide[:, 3:67] = a
+    assert torch.equal(flag_gems.w8a8_int8_grouped_mm(wide[:, 3:67], b, a_s, b_s, offs), want)
+    assert torch.equal(flag_gems.w8a8_int8_grouped_mm(a, b.transpose(1, 2).contiguous().transpose(1, 2), a_s, b_s, offs), want)
+
+
+def test_grouped_nothing_to_compute():
+    a, b, a_s, b_s, offs, _ = _grouped([0, 0], 32, 64)
+    assert flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs).shape == (0, 32)
+    a, b, a_s, b_s, offs, _ = _grouped([4], 32, 64)
+    got = flag_gems.w8a8_int8_grouped_mm(a, b[:0], a_s, b_s[:0], offs[:0])
+    assert got.shape == (4, 32) and not got.any()
+
+
+# ---- quantisation -----------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 8), (3, 264), (2, 5, 4096), (64, 7168)])
+def test_per_token_quant_int8(dtype, shape):
+    x = torch.randn(*shape, generator=torch.Generator().manual_seed(1)).to(dtype)
+    x[..., 0, :] = 0
+    q, s = flag_gems.per_token_quant_int8(x.cuda())
+    assert q.dtype == I8 and q.shape == x.shape and s.shape == x.shape[:-1] + (1,)
+    want_s = x.float().abs().amax(-1, keepdim=True).clamp_min(1e-10) / 127.0
+    assert torch.equal(s.cpu(), want_s)
+    assert torch.equal(q.cpu(), (x.float() / want_s).round().clamp(-128, 127).to(I8))
+    q2, s2 = flag_gems.moe_kernel_quantize_input(x.cuda(), None, I8, True)
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
+def test_per_token_quant_int8_of_a_transposed_matrix():
+    x = torch.randn(64, 40, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    for y, z in zip(flag_gems.per_token_quant_int8(x.t()), flag_gems.per_token_quant_int8(x.t().contiguous())):
+        assert torch.equal(y, z)
+    assert flag_gems.per_token_quant_int8(x[:0])[0].shape == (0, 40)
+
+
+# ---- how they are called ------------------------------------------------------------------------
+class _Off:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_native_and_python_host_paths_agree(monkeypatch):
+    a, b, a_s, b_s, g = _operands(33, 96, 64)
+    ga, gb, ga_s, gb_s, offs, _ = _grouped([9, 0, 140], 96, 64)
+    bias = torch.randn(96, device="cuda", generator=g)
+    x = torch.randn(5, 64, device="cuda", generator=g)
+    c = torch.empty(33, 96, dtype=torch.float16, device="cuda")
+
+    def calls():
+        flag_gems.cutlass_scaled_mm(c, a, b.t(), a_s, b_s, bias.half())
+        return [c.clone(), flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, bias), flag_gems.w8a8_int8_matmul(a[:1], b, a_s[:1], b_s[:1]),
+                flag_gems.w8a8_int8_grouped_mm(ga, gb, ga_s, gb_s, offs, None, torch.float16), *flag_gems.per_token_quant_int8(x)]
+
+    native = calls()
+    monkeypatch.setattr(_cabi, "host", _Off())
+    for u, v in zip(native, calls()):
+        assert u.dtype == v.dtype and torch.equal(u, v)
+
+
+def test_another_stream_and_graph_capture():
+    a, b, a_s, b_s, _ = _operands(16, 4096, 4096)
+    ga, gb, ga_s, gb_s, offs, _ = _grouped([9, 0, 140], 96, 64)
+    want, gwant = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s), flag_gems.w8a8_int8_grouped_mm(ga, gb, ga_s, gb_s, offs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, ggot = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s), flag_gems.w8a8_int8_grouped_mm(ga, gb, ga_s, gb_s, offs)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(ggot, gwant)
+    graphs = []
+    for _ in range(2):  # two graphs of the same call, each with its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            q, s = flag_gems.per_token_quant_int8(a_s.expand(16, 4096).contiguous())
+            out = (flag_gems.w8a8_int8_matmul(a, b, a_s, b_s), flag_gems.w8a8_int8_grouped_mm(ga, gb, ga_s, gb_s, offs), q)
+        graphs.append((graph, out))
+    offs.copy_(torch.tensor([0, 100, 149], device="cuda"))
+    a.copy_(a.roll(1, 0))
+    for graph, _ in graphs:
+        graph.replay()
+    for _, out in graphs:
+        assert torch.equal(out[0], flag_gems.w8a8_int8_matmul(a, b, a_s, b_s))
+        assert torch.equal(out[1], flag_gems.w8a8_int8_grouped_mm(ga, gb, ga_s, gb_s, offs))
+    assert _cabi.device_status() == 0
