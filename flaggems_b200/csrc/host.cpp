@@ -15,6 +15,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/flaggems_b200.h"
@@ -621,6 +623,196 @@ PyObject* moe_sum(PyObject*, PyObject* const* p, Py_ssize_t n) {
     });
 }
 
+// Raised on any thread (a backward pass runs on the engine's), as _cabi.check would.
+void throw_rc(int rc) {
+    if (rc == FG_OK) return;
+    TORCH_CHECK_NOT_IMPLEMENTED(rc != FG_ERR_UNSUPPORTED, fg_last_error());
+    TORCH_CHECK(false, "flaggems_b200 error ", rc, ": ", fg_last_error());
+}
+
+// [rows, values] with the values of a row contiguous, copied only if they are not.
+at::Tensor row_major(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+
+// As Python's once_differentiable: gradients that somebody might differentiate again say that they cannot be.
+void differentiable_once(torch::autograd::variable_list& grads, bool needed) {
+    if (!needed || !at::GradMode::is_enabled()) return;
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable", (int)grads.size());
+    for (auto& g : grads)
+        if (g.defined()) {
+            g = g.detach();
+            g.set_requires_grad(true);
+        }
+    grads = (*error)(std::move(grads));
+}
+
+at::Tensor unpermuted(const at::Tensor& rows, const at::Tensor& row_of_slot, const at::Tensor& weights) {
+    c10::cuda::CUDAGuard guard(rows.device());
+    const int64_t tokens = row_of_slot.size(0), hidden = rows.size(1);
+    at::Tensor out = empty({tokens, hidden}, rows.scalar_type(), rows);
+    const bool w = weights.defined();
+    throw_rc(fg_moe_unpermute(out.data_ptr(), rows.data_ptr(), static_cast<const int32_t*>(row_of_slot.data_ptr()),
+                              w ? weights.data_ptr() : nullptr, w ? dtype_code(weights.scalar_type()) : 0, tokens,
+                              (int)row_of_slot.size(1), rows.size(0), hidden, rows.stride(0), w ? weights.stride(0) : 0,
+                              dtype_code(rows.scalar_type()), stream_of(rows)));
+    return out;
+}
+
+struct Permuted {
+    at::Tensor rows, row_scale, offs, row_of_slot, slot_of_row;
+};
+
+Permuted permuted(const at::Tensor& x, const at::Tensor& ids, int64_t experts, const at::Tensor* scale, const at::Tensor* map) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t tokens = ids.size(0), topk = ids.size(1), n = tokens * topk, cols = scale ? scale->size(1) : 0;
+    Permuted p;
+    p.rows = empty({n, x.size(1)}, x.scalar_type(), x);
+    if (scale) p.row_scale = empty({n, cols}, ScalarType::Float, x);
+    p.offs = empty({experts}, ScalarType::Int, x);
+    p.row_of_slot = empty({tokens, topk}, ScalarType::Int, x);
+    p.slot_of_row = empty({n}, ScalarType::Int, x);
+    throw_rc(fg_moe_permute(p.rows.data_ptr(), scale ? static_cast<float*>(p.row_scale.data_ptr()) : nullptr,
+                            static_cast<int32_t*>(p.offs.data_ptr()), static_cast<int32_t*>(p.row_of_slot.data_ptr()),
+                            static_cast<int32_t*>(p.slot_of_row.data_ptr()), x.data_ptr(),
+                            scale ? static_cast<const float*>(scale->data_ptr()) : nullptr, ids.data_ptr(),
+                            ids.scalar_type() == ScalarType::Long, map ? static_cast<const int32_t*>(map->data_ptr()) : nullptr,
+                            map ? (int)map->numel() : 0, tokens, (int)topk, (int)experts, x.size(1), (int)x.element_size(),
+                            x.stride(0), cols, scale ? scale->stride(0) : 0, stream_of(x)));
+    return p;
+}
+
+struct PermuteFunction : torch::autograd::Function<PermuteFunction> {
+    // `out` receives what has no gradient
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids, int64_t experts,
+                              const at::Tensor* scale, const at::Tensor* map, Permuted* out) {
+        *out = permuted(x, ids, experts, scale, map);
+        ctx->save_for_backward({out->row_of_slot});
+        return out->rows;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d) {
+        torch::autograd::variable_list grads(6);
+        if (!d[0].defined()) return grads;
+        const bool again = d[0].requires_grad();
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            grads[0] = unpermuted(row_major(d[0]), ctx->get_saved_variables()[0], at::Tensor());
+        }
+        differentiable_once(grads, again);
+        return grads;
+    }
+};
+
+struct UnpermuteFunction : torch::autograd::Function<UnpermuteFunction> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& rows, const at::Tensor& row_of_slot,
+                              const std::optional<at::Tensor>& given) {
+        const at::Tensor weights = given.value_or(at::Tensor());
+        const bool d_w = weights.defined() && weights.requires_grad();
+        ctx->save_for_backward({d_w ? rows : at::Tensor(), row_of_slot, weights});
+        ctx->saved_data["n_rows"] = rows.size(0);
+        at::AutoDispatchBelowADInplaceOrView below;
+        return unpermuted(rows, row_of_slot, weights);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d) {
+        torch::autograd::variable_list grads(3);
+        if (!d[0].defined()) return grads;
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &rows = saved[0], &row_of_slot = saved[1], &weights = saved[2];
+        const bool w = weights.defined(), want_rows = ctx->needs_input_grad(0), want_w = w && ctx->needs_input_grad(2) && rows.defined();
+        const bool again = d[0].requires_grad() || (w && weights.requires_grad()) || (rows.defined() && rows.requires_grad());
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const at::Tensor d_out = row_major(d[0]);
+            c10::cuda::CUDAGuard guard(d_out.device());
+            const int64_t n = ctx->saved_data["n_rows"].toInt(), hidden = d_out.size(1);
+            if (want_rows) grads[0] = empty({n, hidden}, d_out.scalar_type(), d_out);
+            if (want_w) grads[2] = empty(weights.sizes(), weights.scalar_type(), d_out);
+            throw_rc(fg_moe_unpermute_backward(
+                want_rows ? grads[0].data_ptr() : nullptr, want_w ? grads[2].data_ptr() : nullptr, d_out.data_ptr(),
+                want_w ? rows.data_ptr() : nullptr, static_cast<const int32_t*>(row_of_slot.data_ptr()),
+                w ? weights.data_ptr() : nullptr, w ? dtype_code(weights.scalar_type()) : 0, row_of_slot.size(0),
+                (int)row_of_slot.size(1), n, hidden, d_out.stride(0), want_w ? rows.stride(0) : 0, w ? weights.stride(0) : 0,
+                dtype_code(d_out.scalar_type()), stream_of(d_out)));
+        }
+        differentiable_once(grads, again);
+        return grads;
+    }
+};
+
+bool rows_of_values(const at::Tensor& t) { return t.dim() == 2 && (t.stride(1) == 1 || t.size(1) <= 1); }
+
+// moe_permute(x, topk_ids, num_experts, scale or None, expert_map or None) -> (rows, row_scale or None, offs, row_of_slot, slot_of_row)
+PyObject* moe_permute(PyObject*, PyObject* const* p, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        int64_t experts;
+        const at::Tensor *x = n == 5 ? cuda_tensor(p[0]) : nullptr, *ids = x ? cuda_tensor(p[1]) : nullptr;
+        if (!ids || !py_int(p[2], &experts) || experts < 1 || experts > 1024 || !rows_of_values(*x) || ids->dim() != 2) return none();
+        switch (x->scalar_type()) {
+            case ScalarType::BFloat16: case ScalarType::Half: case ScalarType::Float: case ScalarType::Char: case ScalarType::Byte:
+            case E4M3: case ScalarType::Float8_e5m2: break;
+            default: return none();
+        }
+        if (ids->scalar_type() != ScalarType::Int && ids->scalar_type() != ScalarType::Long) return none();
+        if (!ids->is_contiguous() || ids->size(0) != x->size(0) || ids->device() != x->device()) return none();
+        const at::Tensor *scale = nullptr, *map = nullptr;
+        const bool grad = at::GradMode::is_enabled();
+        if (p[3] != Py_None) {
+            scale = cuda_tensor(p[3]);
+            if (!scale || scale->scalar_type() != ScalarType::Float || !rows_of_values(*scale) || scale->size(0) != x->size(0) ||
+                scale->device() != x->device() || (grad && scale->requires_grad()))
+                return none();
+        }
+        if (p[4] != Py_None) {
+            map = cuda_tensor(p[4]);
+            if (!map || map->scalar_type() != ScalarType::Int || map->dim() != 1 || map->numel() == 0 || !map->is_contiguous() ||
+                map->device() != x->device())
+                return none();
+        }
+        Permuted out;
+        unlocked([&] {
+            if (grad && x->requires_grad()) {
+                out.rows = PermuteFunction::apply(*x, *ids, experts, scale, map, &out);
+            } else {
+                out = permuted(*x, *ids, experts, scale, map);
+            }
+            return 0;
+        });
+        PyObject* t = PyTuple_New(5);
+        if (!t) return nullptr;
+        at::Tensor* parts[5] = {&out.rows, &out.row_scale, &out.offs, &out.row_of_slot, &out.slot_of_row};
+        for (int i = 0; i < 5; ++i) {
+            PyObject* o = parts[i]->defined() ? THPVariable_Wrap(std::move(*parts[i])) : none();
+            if (!o) {
+                Py_DECREF(t);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(t, i, o);
+        }
+        return t;
+    });
+}
+
+// moe_unpermute(rows, row_of_slot, weights or None) -> out
+PyObject* moe_unpermute(PyObject*, PyObject* const* p, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const at::Tensor *rows = n == 3 ? cuda_tensor(p[0]) : nullptr, *slots = rows ? cuda_tensor(p[1]) : nullptr;
+        if (!slots || dtype_code(rows->scalar_type()) < 0 || !rows_of_values(*rows) || slots->scalar_type() != ScalarType::Int ||
+            slots->dim() != 2 || !slots->is_contiguous() || slots->device() != rows->device() || slots->numel() != rows->size(0))
+            return none();
+        at::Tensor weights;
+        if (p[2] != Py_None) {
+            const at::Tensor* w = cuda_tensor(p[2]);
+            if (!w || dtype_code(w->scalar_type()) < 0 || w->sizes() != slots->sizes() || !rows_of_values(*w) ||
+                w->device() != rows->device())
+                return none();
+            weights = *w;
+        }
+        const bool grad = at::GradMode::is_enabled() && (rows->requires_grad() || (weights.defined() && weights.requires_grad()));
+        return THPVariable_Wrap(unlocked(
+            [&] { return grad ? UnpermuteFunction::apply(*rows, *slots, weights.defined() ? std::optional<at::Tensor>(weights) : std::nullopt)
+                                : unpermuted(*rows, *slots, weights); }));
+    });
+}
+
 // fused_experts(hidden, w1, w2, topk_weights, topk_ids, out, mode, w1_scale, w2_scale, a1_scale, a2_scale,
 //               num_experts, expert_map, tokens per chunk) -> out.  The caller has checked shapes, types and
 // layouts; scales, map and the two activation scales may be None.
@@ -673,7 +865,7 @@ PyObject* fused_experts(PyObject*, PyObject* const* p, Py_ssize_t n) {
 PyMethodDef methods[] = {
     FG_METHOD(group_quant), FG_METHOD(act_quant),    FG_METHOD(token_quant), FG_METHOD(tensor_quant),
     FG_METHOD(block_mm),    FG_METHOD(scaled_mm),    FG_METHOD(scaled_mm_new), FG_METHOD(grouped_mm),
-    FG_METHOD(token_quant_int8), FG_METHOD(int8_mm), FG_METHOD(int8_grouped_mm),
+    FG_METHOD(moe_permute), FG_METHOD(moe_unpermute), FG_METHOD(token_quant_int8), FG_METHOD(int8_mm), FG_METHOD(int8_grouped_mm),
     FG_METHOD(topk_softmax), FG_METHOD(grouped_topk), FG_METHOD(moe_align),  FG_METHOD(silu_mul),
     FG_METHOD(moe_sum),     FG_METHOD(fused_experts), {nullptr, nullptr, 0, nullptr}};
 

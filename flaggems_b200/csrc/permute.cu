@@ -10,6 +10,7 @@
 #include <cooperative_groups.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -39,9 +40,14 @@ __device__ __forceinline__ int expert_of(const SortArgs& a, int64_t i) {
     return id >= 0 && id < a.num_experts ? (int)id : a.num_experts;
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // A counting sort by one cluster, stable like a sort by (expert, slot): every warp owns a contiguous segment of
 // the slots and counts it, the counts are scanned over warps, CTAs (distributed shared memory) and experts, and every warp
 // walks its segment again in order.  Bucket num_experts takes the slots without an expert.
+// SEG > 0: segments of up to 32 * SEG slots stay in registers between the two walks and are loaded all at once.
+template <int SEG>
 __global__ void __launch_bounds__(SORT_THREADS, 1) sort_slots_kernel(SortArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
@@ -54,23 +60,35 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_slots_kernel(SortArgs a)
     int32_t* cta_total = smem + SORT_WARPS * B;   // [B] read by the other CTAs
     int32_t* base = cta_total + B;                // [B] first row of this CTA
     __shared__ int32_t scan_tmp[SORT_WARPS];
-    for (int i = threadIdx.x; i < SORT_WARPS * B; i += SORT_THREADS) warp_hist[i] = 0;
-    __syncthreads();
 
     const int64_t segments = (int64_t)n_ranks * SORT_WARPS;
     const int64_t seg_len = ((a.numel + segments - 1) / segments + 31) / 32 * 32;
     const int64_t seg_begin = min((rank * (int64_t)SORT_WARPS + warp) * seg_len, a.numel);
     const int64_t seg_end = min(seg_begin + seg_len, a.numel);
+    auto bucket = [&](int64_t i) -> int { return i < seg_end ? expert_of(a, i) : -1; };
+    int kept[SEG > 0 ? SEG : 1];
+    if constexpr (SEG > 0) {
+#pragma unroll
+        for (int c = 0; c < SEG; ++c) kept[c] = bucket(seg_begin + 32 * c + lane);
+    }
+    for (int i = threadIdx.x; i < SORT_WARPS * B; i += SORT_THREADS) warp_hist[i] = 0;
+    __syncthreads();
+
     int32_t* my_hist = warp_hist + warp * B;
-    for (int64_t i0 = seg_begin; i0 < seg_end; i0 += 32) {
-        const int e = i0 + lane < seg_end ? expert_of(a, i0 + lane) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && lane == __ffs(peers) - 1) my_hist[e] += __popc(peers);
-        __syncwarp();
+    auto count = [&](int e) {
+        if (e >= 0) atomicAdd(&my_hist[e], 1);
+    };
+    if constexpr (SEG > 0) {
+#pragma unroll
+        for (int c = 0; c < SEG; ++c)
+            if (seg_begin + 32 * c < seg_end) count(kept[c]);
+    } else {
+        for (int64_t i0 = seg_begin; i0 < seg_end; i0 += 32) count(bucket(i0 + lane));
     }
     __syncthreads();
     for (int e = threadIdx.x; e < B; e += SORT_THREADS) {
         int32_t run = 0;
+#pragma unroll
         for (int w = 0; w < SORT_WARPS; ++w) {
             const int32_t t = warp_hist[w * B + e];
             warp_hist[w * B + e] = run;
@@ -82,6 +100,7 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_slots_kernel(SortArgs a)
     const int e0 = threadIdx.x;  // num_experts <= SORT_THREADS; the last bucket follows all others and needs no scan
     int32_t before = 0, total = 0;
     if (e0 < E) {
+#pragma unroll 8
         for (int r = 0; r < n_ranks; ++r) {
             const int32_t c = cluster.map_shared_rank(cta_total, r)[e0];
             if (r < rank) before += c;
@@ -91,7 +110,7 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_slots_kernel(SortArgs a)
     int32_t none_before = 0;
     if (threadIdx.x == 0)
         for (int r = 0; r < rank; ++r) none_before += cluster.map_shared_rank(cta_total, r)[E];
-    cluster.sync();  // nobody leaves while the others read its counts
+    cluster_arrive();  // nobody leaves while the others read its counts
     int32_t incl = total;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -117,50 +136,182 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_slots_kernel(SortArgs a)
     }
     if (threadIdx.x == 0) base[E] = scan_tmp[SORT_WARPS - 1] + none_before;
     __syncthreads();
-    for (int64_t i0 = seg_begin; i0 < seg_end; i0 += 32) {
-        const int64_t i = i0 + lane;
-        const int e = i < seg_end ? expert_of(a, i) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, e);
-        const int leader = __ffs(peers) - 1;
-        int32_t cur = 0;
-        if (e >= 0 && lane == leader) {
-            cur = my_hist[e];
-            my_hist[e] = cur + __popc(peers);
+    const int bits = 32 - __clz(E);
+    auto place = [&](int64_t i, int e) {
+        // lanes of the same bucket, one vote per bit of the bucket's number (a match over 32 lanes of many different
+        // buckets takes several times as long)
+        unsigned peers = __ballot_sync(0xffffffffu, e >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned ones = __ballot_sync(0xffffffffu, (e >> b) & 1);
+            peers &= (e >> b) & 1 ? ones : ~ones;
         }
-        cur = __shfl_sync(0xffffffffu, cur, leader);
+        const int32_t cur = e >= 0 ? my_hist[e] : 0;
+        __syncwarp();
         if (e >= 0) {
-            const int32_t row = base[e] + cur + __popc(peers & ((1u << lane) - 1u));
+            const unsigned below = peers & ((1u << lane) - 1u);
+            if (below == 0u) my_hist[e] = cur + __popc(peers);
+            const int32_t row = base[e] + cur + __popc(below);
             a.row_of_slot[i] = e < E ? row : ~row;
             a.slot_of_row[row] = (int32_t)i;
         }
         __syncwarp();
+    };
+    if constexpr (SEG > 0) {
+#pragma unroll
+        for (int c = 0; c < SEG; ++c)
+            if (seg_begin + 32 * c < seg_end) place(seg_begin + 32 * c + lane, kept[c]);
+    } else {
+        for (int64_t i0 = seg_begin; i0 < seg_end; i0 += 32) place(i0 + lane, bucket(i0 + lane));
+    }
+    cluster_wait();
+}
+
+// A token's row to the rows of its slots; rows of slots without an expert become zeros (their scales 1).
+struct RowArgs {
+    const void* x;
+    int64_t ld_x;  // units
+    const float* scale;
+    int64_t ld_scale;
+    int topk;
+    int64_t n_rows;
+    void* rows;
+    int units;  // per row
+    float* row_scale;
+    int scale_cols;
+};
+constexpr int SLOTS_AT_ONCE = 8;
+
+template <typename UNIT, int N>
+__device__ __forceinline__ void load_pieces(const RowArgs& a, int64_t t, int v0, UNIT (&piece)[N]) {
+    const UNIT* x = reinterpret_cast<const UNIT*>(a.x) + t * a.ld_x;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int v = v0 + u * (int)blockDim.x;
+        piece[u] = v < a.units ? x[v] : UNIT{};
     }
 }
 
-// One CTA per token: its row is read once and written to the rows of its slots; rows of slots without an expert
-// become zeros (their scales 1).  UNIT: the bytes of a load, 16 where everything is aligned to that.
+template <typename UNIT, int N>
+__device__ __forceinline__ void store_pieces(const RowArgs& a, int32_t r, int v0, const UNIT (&piece)[N]) {
+    const int64_t row = r < 0 ? ~r : r;
+    if (row >= a.n_rows) return;
+    UNIT* out = reinterpret_cast<UNIT*>(a.rows) + row * a.units;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int v = v0 + u * (int)blockDim.x;
+        if (v < a.units) out[v] = r < 0 ? UNIT{} : piece[u];
+    }
+}
+
+__device__ __forceinline__ void store_scales(const RowArgs& a, int64_t t, int k, int32_t r) {
+    const int64_t row = r < 0 ? ~r : r;
+    if (row >= a.n_rows) return;
+    for (int c = threadIdx.x; c < a.scale_cols; c += blockDim.x)
+        a.row_scale[row * a.scale_cols + c] = r < 0 ? 1.0f : a.scale[t * a.ld_scale + c];
+}
+
+// One CTA per token: its row is read once, two pieces per thread, and written slot after slot.  Bound by the writes, which
+// are topk times the reads.  Few registers (and so many CTAs, a row each, under way) matter more than pieces per
+// thread: 8192 x 8 rows of 7168 bytes take 88 us this way, 98 with four pieces and the slots' rows in registers, 91-97 as
+// bulk copies through a ring in shared memory (6.0 TB/s of the 6.6 of a copy).
+// UNIT: the bytes of a load, 16 where everything is aligned to that.
 template <typename UNIT>
-__global__ void __launch_bounds__(256) permute_rows_kernel(const UNIT* x, int64_t ld_x, const float* scale, int64_t ld_scale,
-                                                           const int32_t* row_of_slot, int topk, int64_t n_rows, UNIT* rows,
-                                                           int units, float* row_scale, int scale_cols) {
+__global__ void __launch_bounds__(256) permute_rows_kernel(RowArgs a, const int32_t* row_of_slot) {
     fg_pdl_wait();
     fg_pdl_trigger();
+    constexpr int PIECES = 2;
     const int64_t t = blockIdx.x;
-    for (int v = threadIdx.x; v < units; v += blockDim.x) {
-        const UNIT value = x[t * ld_x + v];
-        for (int k = 0; k < topk; ++k) {
-            const int32_t r = row_of_slot[t * topk + k];
-            const int64_t row = r < 0 ? ~r : r;
-            if (row < n_rows) rows[row * units + v] = r < 0 ? UNIT{} : value;
-        }
+    for (int v0 = threadIdx.x; v0 < a.units; v0 += PIECES * blockDim.x) {
+        UNIT piece[PIECES];
+        load_pieces(a, t, v0, piece);
+#pragma unroll 1
+        for (int k = 0; k < a.topk; ++k) store_pieces(a, row_of_slot[t * a.topk + k], v0, piece);
     }
-    for (int c = threadIdx.x; c < scale_cols; c += blockDim.x) {
-        const float value = scale[t * ld_scale + c];
-        for (int k = 0; k < topk; ++k) {
-            const int32_t r = row_of_slot[t * topk + k];
-            const int64_t row = r < 0 ? ~r : r;
-            if (row < n_rows) row_scale[row * scale_cols + c] = r < 0 ? 1.0f : value;
+    if (a.scale_cols)
+        for (int k = 0; k < a.topk; ++k) store_scales(a, t, k, row_of_slot[t * a.topk + k]);
+}
+
+// Few slots: sorting and copying in one launch.  The CTA of a token counts for each of its slots the slots that come
+// before it in (expert, slot) order, which is the slot's row, while the token's row is on its way.  The last
+// CTA counts the experts instead.
+template <typename UNIT>
+__global__ void __launch_bounds__(256) sort_and_permute_kernel(SortArgs s, RowArgs a) {
+    fg_pdl_wait();
+    fg_pdl_trigger();
+    constexpr int PIECES = 4;
+    __shared__ int32_t hist[SORT_THREADS];
+    __shared__ int32_t before[8][SLOTS_AT_ONCE];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int numel = (int)s.numel, E = s.num_experts;
+    const int64_t t = blockIdx.x;
+    if (t * a.topk >= numel) {
+        for (int e = threadIdx.x; e < E; e += blockDim.x) hist[e] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < numel; i += blockDim.x) {
+            const int e = expert_of(s, i);
+            if (e < E) atomicAdd(&hist[e], 1);
         }
+        __syncthreads();
+        if (warp == 0) {
+            int32_t run = 0;
+            for (int e0 = 0; e0 < E; e0 += 32) {
+                int32_t incl = e0 + lane < E ? hist[e0 + lane] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                if (e0 + lane < E) s.offs[e0 + lane] = run + incl;
+                run += __shfl_sync(0xffffffffu, incl, 31);
+            }
+        }
+        return;
+    }
+    UNIT piece[PIECES];
+    const int v0 = threadIdx.x;
+    load_pieces(a, t, v0, piece);
+    for (int k0 = 0; k0 < a.topk; k0 += SLOTS_AT_ONCE) {
+        const int first = (int)t * a.topk + k0;
+        // (expert, slot) as one number: fits because numel * (num_experts + 1) < 2^31 here
+        int32_t key[SLOTS_AT_ONCE], n[SLOTS_AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < SLOTS_AT_ONCE; ++k) {
+            key[k] = k0 + k < a.topk ? expert_of(s, first + k) * numel + first + k : 0;
+            n[k] = 0;
+        }
+#pragma unroll 2
+        for (int i = threadIdx.x; i < numel; i += blockDim.x) {
+            const int32_t other = expert_of(s, i) * numel + i;
+#pragma unroll
+            for (int k = 0; k < SLOTS_AT_ONCE; ++k) n[k] += other < key[k];
+        }
+#pragma unroll
+        for (int k = 0; k < SLOTS_AT_ONCE; ++k) {
+            const int32_t sum = __reduce_add_sync(0xffffffffu, n[k]);
+            if (lane == 0) before[warp][k] = sum;
+        }
+        __syncthreads();
+        int32_t r[SLOTS_AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < SLOTS_AT_ONCE; ++k) {
+            r[k] = 0;
+            for (int w = 0; w < warps; ++w) r[k] += before[w][k];
+            if (k0 + k >= a.topk) continue;
+            const bool none = key[k] >= E * numel;
+            if (threadIdx.x == 0) {
+                s.slot_of_row[r[k]] = first + k;
+                s.row_of_slot[first + k] = none ? ~r[k] : r[k];
+            }
+            if (none) r[k] = ~r[k];
+            store_pieces(a, r[k], v0, piece);
+            for (int v = v0 + PIECES * blockDim.x; v < a.units; v += PIECES * blockDim.x) {  // rows of more than 16 KB
+                UNIT more[PIECES];
+                load_pieces(a, t, v, more);
+                store_pieces(a, r[k], v, more);
+            }
+            if (a.scale_cols) store_scales(a, t, k0 + k, r[k]);
+        }
+        __syncthreads();
     }
 }
 
@@ -193,76 +344,166 @@ struct SumArgs {
     void* d_w;     // [T, topk]; NULL: not wanted
 };
 
-// One CTA per token; sums in fp32 in slot order.
+// V consecutive values of a row: one 16-byte load, or one value where rows are not aligned to that.
 template <typename T, int V>
+struct Piece {
+    static_assert(V == 1 || V * sizeof(T) == 16, "one value or 16 bytes");
+    using Raw = std::conditional_t<V == 1, T, uint4>;
+    static __device__ __forceinline__ Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+    static __device__ __forceinline__ Raw load_once(const T* p) {
+        if constexpr (V == 1) return *p;
+        else return __ldcs(reinterpret_cast<const uint4*>(p));
+    }
+    static __device__ __forceinline__ void unpack(const Raw& raw, float (&f)[V]) {
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = fg_to_float(e[i]);
+    }
+    static __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
+        Raw raw;
+        T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < V; ++i) e[i] = fg_from_float<T>(f[i]);
+        *reinterpret_cast<Raw*>(p) = raw;
+    }
+};
+
+// Rows and weights of K consecutive slots of token t; row -1: nothing to read.
+template <int K>
+__device__ __forceinline__ void load_slots(const SumArgs& a, int64_t t, int k0, int32_t (&row)[K], float (&w)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        row[k] = k0 + k < a.topk ? a.row_of_slot[t * a.topk + k0 + k] : -1;
+        w[k] = a.weights && k0 + k < a.topk ? load_weight(a.weights, a.w_dtype, t * a.ld_w + k0 + k) : 1.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (row[k] < 0 || row[k] >= a.n_rows) row[k] = -1;
+}
+
+// One CTA per token (and per part of its columns, blockIdx.y), sums in fp32 in slot order.  A thread has K slots
+// of U pieces in flight, eight loads whatever the number of slots.
+template <typename T, int V, int K>
 __global__ void __launch_bounds__(256) unpermute_kernel(SumArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
+    constexpr int U = K >= 8 ? 1 : 8 / K;
+    using P = Piece<T, V>;
     const int64_t t = blockIdx.x;
     const T* rows = reinterpret_cast<const T*>(a.rows);
-    for (int64_t c = (int64_t)threadIdx.x * V; c < a.H; c += (int64_t)blockDim.x * V) {
-        float acc[V];
+    const int64_t step = (int64_t)blockDim.x * V;
+    int32_t row[K];
+    float w[K];
+    load_slots(a, t, 0, row, w);
+    for (int64_t c = ((int64_t)blockIdx.y * U * blockDim.x + threadIdx.x) * V; c < a.H; c += gridDim.y * U * step) {
+        float acc[U][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-        for (int k = 0; k < a.topk; ++k) {
-            const int32_t r = a.row_of_slot[t * a.topk + k];
-            if (r < 0 || r >= a.n_rows) continue;
-            const float w = a.weights ? load_weight(a.weights, a.w_dtype, t * a.ld_w + k) : 1.0f;
-            float f[V];
-            if constexpr (V == 8) fg_load8(rows + r * a.ld_rows + c, f);
-            else f[0] = fg_to_float(rows[r * a.ld_rows + c]);
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = fmaf(w, f[i], acc[i]);
+            for (int i = 0; i < V; ++i) acc[u][i] = 0.0f;
+        for (int k0 = 0;;) {
+            typename P::Raw raw[K][U];
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (row[k] >= 0 && c + u * step < a.H) raw[k][u] = P::load_once(rows + row[k] * a.ld_rows + c + u * step);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (row[k] < 0) continue;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float f[V];
+                    P::unpack(raw[k][u], f);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[u][i] = fmaf(w[k], f[i], acc[u][i]);
+                }
+            }
+            if (a.topk <= K) break;  // the slots stay in registers
+            k0 = k0 + K < a.topk ? k0 + K : 0;
+            load_slots(a, t, k0, row, w);
+            if (k0 == 0) break;
         }
-        T* out = reinterpret_cast<T*>(a.out) + t * a.H + c;
-        if constexpr (V == 8) fg_store8(out, acc);
-        else out[0] = fg_from_float<T>(acc[0]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c + u * step < a.H) P::store(reinterpret_cast<T*>(a.out) + t * a.H + c + u * step, acc[u]);
     }
 }
 
-// One CTA per token: d_out[t] times the weight into the gradient of every row of the token, and its product
-// with the row summed over the CTA into the gradient of the weight.
+// One CTA per token: d_out[t] times the weight into the gradient of every row of the token, and its product with
+// the row into the gradient of the weight, slot after slot.  d_out is read once where a row is up to four pieces per
+// thread (16 KB), everything else is read and written once; the products are summed in a fixed order: a thread's columns, the
+// lanes, the warps.  Bound by HBM: 8192 x 8 bf16 rows of 7168 (2.0 GB) take 307 us, 6.5 TB/s, which is the rate of a
+// copy.  More slots in flight per thread cost registers and with them CTAs (404 us with two slots at once); streaming
+// loads and stores (.cs) take 315.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) unpermute_backward_kernel(SumArgs a) {
+__global__ void __launch_bounds__(256, 4) unpermute_backward_kernel(SumArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
-    __shared__ float part[8];
+    constexpr int U = 4, K = 32;  // pieces per thread and round, slots whose sums are parked at once
+    using P = Piece<T, V>;
+    __shared__ float part[8][K];
     const int64_t t = blockIdx.x;
     const T* rows = reinterpret_cast<const T*>(a.rows);
     const T* d_out = reinterpret_cast<const T*>(a.d_out) + t * a.ld_d_out;
-    for (int k = 0; k < a.topk; ++k) {
-        const int32_t r = a.row_of_slot[t * a.topk + k];
-        const int64_t row = r < 0 ? ~r : r;
-        const bool inside = row < a.n_rows, real = r >= 0 && inside;
-        const float w = real && a.weights ? load_weight(a.weights, a.w_dtype, t * a.ld_w + k) : 1.0f;
-        float dot = 0.0f;
-        for (int64_t c = (int64_t)threadIdx.x * V; c < a.H; c += (int64_t)blockDim.x * V) {
-            float g[V], f[V];
-            if constexpr (V == 8) fg_load8(d_out + c, g);
-            else g[0] = fg_to_float(d_out[c]);
-            if (a.d_w && real) {
-                if constexpr (V == 8) fg_load8(rows + row * a.ld_rows + c, f);
-                else f[0] = fg_to_float(rows[row * a.ld_rows + c]);
+    T* d_rows = reinterpret_cast<T*>(a.d_rows);
+    const int step = (int)blockDim.x * V, first = (int)threadIdx.x * V, H = (int)a.H;
+    const bool one_round = H <= U * step;
+    typename P::Raw g[U];
+    auto load_g = [&](int c) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) dot = fmaf(g[i], f[i], dot);
+        for (int u = 0; u < U; ++u)
+            if (c + u * step < H) g[u] = P::load(d_out + c + u * step);
+    };
+    if (one_round) load_g(first);
+    for (int k0 = 0; k0 < a.topk; k0 += K) {
+        const int slots = min(K, a.topk - k0);
+#pragma unroll 1
+        for (int k = 0; k < slots; ++k) {
+            const int32_t r = a.row_of_slot[t * a.topk + k0 + k];
+            const int64_t row = r < 0 ? ~r : r;
+            const bool real = r >= 0 && row < a.n_rows;
+            const float w = real && a.weights ? load_weight(a.weights, a.w_dtype, t * a.ld_w + k0 + k) : 1.0f;
+            const T* from = rows + row * a.ld_rows;
+            T* to = a.d_rows && row < a.n_rows ? d_rows + row * a.H : nullptr;
+            float dot = 0.0f;
+            for (int c = first; c < H; c += U * step) {
+                if (!one_round) load_g(c);
+                typename P::Raw raw[U];
+                if (a.d_w && real) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (c + u * step < H) raw[u] = P::load(from + c + u * step);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (c + u * step >= H) continue;
+                    float f[V], x[V];
+                    P::unpack(g[u], f);
+                    if (a.d_w && real) {
+                        P::unpack(raw[u], x);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) dot = fmaf(f[i], x[i], dot);
+                    }
+                    if (to) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) f[i] = real ? w * f[i] : 0.0f;
+                        P::store(to + c + u * step, f);
+                    }
+                }
             }
-            if (a.d_rows && inside) {
+            if (a.d_w) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) g[i] = real ? w * g[i] : 0.0f;
-                T* o = reinterpret_cast<T*>(a.d_rows) + row * a.H + c;
-                if constexpr (V == 8) fg_store8(o, g);
-                else o[0] = fg_from_float<T>(g[0]);
+                for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+                if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][k] = dot;
             }
         }
         if (a.d_w) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
             __syncthreads();
-            if (threadIdx.x == 0) {
+            if ((int)threadIdx.x < slots) {
                 float sum = 0.0f;
-                for (int i = 0; i < (int)blockDim.x / 32; ++i) sum += part[i];
-                store_weight(a.d_w, a.w_dtype, t * a.topk + k, real ? sum : 0.0f);
+                for (int i = 0; i < (int)blockDim.x / 32; ++i) sum += part[i][threadIdx.x];
+                store_weight(a.d_w, a.w_dtype, t * a.topk + k0 + threadIdx.x, sum);
             }
             __syncthreads();
         }
@@ -286,6 +527,30 @@ unsigned threads_for(int64_t n) { return n >= 256 ? 256u : (unsigned)(n < 32 ? 3
 
 bool aligned16(const void* p, int64_t stride_bytes) { return (uintptr_t)p % 16 == 0 && stride_bytes % 16 == 0; }
 
+// Up to here every token's CTA looks at all slots for itself.
+constexpr int64_t ONE_LAUNCH_SLOTS = 4096;
+
+int sort_slots(const SortArgs& a, cudaStream_t st) {
+    int ranks = 1;
+    while (ranks < 8 && (int64_t)ranks * SORT_THREADS * 2 < a.numel) ranks *= 2;
+    const size_t smem = (size_t)(SORT_WARPS + 2) * (a.num_experts + 1) * sizeof(int32_t);
+    const bool kept = fg_cdiv(a.numel, (int64_t)ranks * SORT_THREADS) <= 8;
+    auto kernel = kept ? sort_slots_kernel<8> : sort_slots_kernel<0>;
+    static std::mutex mu;
+    static size_t smem_set[64][2];
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        size_t& have = smem_set[fg_device_index()][kept];
+        if (have < 48 * 1024) have = 48 * 1024;
+        if (smem > have) {
+            FG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            have = smem;
+        }
+    }
+    FG_CUDA(fg_launch(kernel, (unsigned)ranks, SORT_THREADS, smem, st, (unsigned)ranks, a));
+    return FG_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -306,32 +571,21 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
     FG_REQUIRE(numel == 0 || scale_cols == 0 || (row_scale && scale), FG_ERR_INVALID_ARGUMENT, "null pointer");
     cudaStream_t st = (cudaStream_t)stream;
     const SortArgs a{topk_ids, ids_are_i64, numel, num_experts, expert_map, expert_map_len, offs, row_of_slot, slot_of_row};
-    int ranks = 1;
-    while (ranks < 8 && (int64_t)ranks * SORT_THREADS * 4 < numel) ranks *= 2;
-    const size_t smem = (size_t)(SORT_WARPS + 2) * (num_experts + 1) * sizeof(int32_t);
-    static std::mutex mu;
-    static size_t smem_set[64];
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        size_t& have = smem_set[fg_device_index()];
-        if (have < 48 * 1024) have = 48 * 1024;
-        if (smem > have) {
-            FG_CUDA(cudaFuncSetAttribute(sort_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            have = smem;
-        }
-    }
-    FG_CUDA(fg_launch(sort_slots_kernel, (unsigned)ranks, SORT_THREADS, smem, st, (unsigned)ranks, a));
-    if (numel == 0 || (H == 0 && scale_cols == 0)) return FG_OK;
     const int64_t row_bytes = H * elem_bytes;
-    auto go = [&](auto unit) -> cudaError_t {
-        using U = decltype(unit);
-        const int64_t units = row_bytes / (int64_t)sizeof(U);
-        return fg_launch(permute_rows_kernel<U>, (unsigned)T, threads_for(units), 0, st, 1, (const U*)x,
-                         ld_x * elem_bytes / (int64_t)sizeof(U), scale, ld_scale, (const int32_t*)row_of_slot, topk, numel, (U*)rows,
-                         (int)units, row_scale, (int)scale_cols);
-    };
     const bool vec = aligned16(x, ld_x * elem_bytes) && aligned16(rows, row_bytes);
-    FG_CUDA(vec ? go(uint4()) : elem_bytes == 4 ? go(uint32_t()) : elem_bytes == 2 ? go(uint16_t()) : go(uint8_t()));
+    const int unit = vec ? 16 : elem_bytes;
+    const RowArgs r{x, ld_x * elem_bytes / unit, scale, ld_scale, topk, numel, rows, (int)(row_bytes / unit), row_scale, (int)scale_cols};
+    const unsigned threads = threads_for(r.units);
+    auto by_unit = [&](auto&& go) -> cudaError_t {
+        return vec ? go(uint4()) : elem_bytes == 4 ? go((unsigned int)0) : elem_bytes == 2 ? go((unsigned short)0) : go((unsigned char)0);
+    };
+    if (numel > 0 && numel <= ONE_LAUNCH_SLOTS) {
+        FG_CUDA(by_unit([&](auto u) { return fg_launch(sort_and_permute_kernel<decltype(u)>, (unsigned)T + 1, threads < 128 ? 128u : threads, 0, st, 1, a, r); }));
+        return FG_OK;
+    }
+    const int rc = sort_slots(a, st);
+    if (rc != FG_OK || numel == 0 || (H == 0 && scale_cols == 0)) return rc;
+    FG_CUDA(by_unit([&](auto u) { return fg_launch(permute_rows_kernel<decltype(u)>, (unsigned)T, threads, 0, st, 1, r, (const int32_t*)row_of_slot); }));
     return FG_OK;
 }
 
@@ -347,11 +601,20 @@ int fg_moe_unpermute(void* out, const void* rows, const int32_t* row_of_slot, co
     a.rows = rows; a.ld_rows = ld_rows; a.n_rows = n_rows; a.row_of_slot = row_of_slot; a.weights = weights; a.w_dtype = w_dtype;
     a.ld_w = ld_w; a.topk = topk; a.H = H; a.out = out;
     const int es = elem_size(dtype);
-    const bool vec = H % 8 == 0 && aligned16(rows, ld_rows * es) && aligned16(out, H * es);
+    const bool vec = aligned16(rows, ld_rows * es) && aligned16(out, H * es);
+    const int slots = topk <= 2 ? 2 : topk <= 4 ? 4 : 8;  // at once
+    const int64_t pieces = fg_cdiv(vec ? H * es / 16 : H, 8 / slots);  // per thread: 8 / slots
+    // Few tokens: their columns are spread over CTAs, until there are two CTAs per SM or a thread has one round.
+    unsigned parts = 1;
+    while (parts < 64 && T * parts < 2 * fg_num_sms() && parts * (int64_t)threads_for(pieces) < pieces) parts *= 2;
     return by_type(dtype, [&](auto tag) -> int {
         using E = decltype(tag);
-        FG_CUDA(vec ? fg_launch(unpermute_kernel<E, 8>, (unsigned)T, threads_for(H / 8), 0, (cudaStream_t)stream, 1, a)
-                    : fg_launch(unpermute_kernel<E, 1>, (unsigned)T, threads_for(H), 0, (cudaStream_t)stream, 1, a));
+        auto go = [&](auto kernel) { return fg_launch(kernel, dim3((unsigned)T, parts), threads_for(pieces), 0, (cudaStream_t)stream, 1, a); };
+        auto by_slots = [&](auto v) -> cudaError_t {
+            constexpr int V = decltype(v)::value;
+            return slots == 2 ? go(unpermute_kernel<E, V, 2>) : slots == 4 ? go(unpermute_kernel<E, V, 4>) : go(unpermute_kernel<E, V, 8>);
+        };
+        FG_CUDA(vec ? by_slots(std::integral_constant<int, 16 / sizeof(E)>()) : by_slots(std::integral_constant<int, 1>()));
         return FG_OK;
     });
 }
@@ -360,7 +623,7 @@ int fg_moe_unpermute_backward(void* d_rows, void* d_weights, const void* d_out, 
                               const void* weights, int w_dtype, int64_t T, int topk, int64_t n_rows, int64_t H, int64_t ld_d_out,
                               int64_t ld_rows, int64_t ld_w, int dtype, void* stream) {
     FG_REQUIRE(T >= 0 && topk >= 0 && n_rows >= 0 && H >= 0, FG_ERR_INVALID_ARGUMENT, "negative size");
-    FG_REQUIRE(T < (1ll << 31) && n_rows < (1ll << 31), FG_ERR_UNSUPPORTED, "size too large");
+    FG_REQUIRE(T < (1ll << 31) && n_rows < (1ll << 31) && H < (1ll << 30), FG_ERR_UNSUPPORTED, "size too large");
     FG_REQUIRE(!(weights || d_weights) || w_dtype == FG_DTYPE_BF16 || w_dtype == FG_DTYPE_F16 || w_dtype == FG_DTYPE_F32,
                FG_ERR_INVALID_ARGUMENT, "bad weight dtype %d", w_dtype);
     if (T == 0 || topk == 0) return FG_OK;
@@ -369,10 +632,11 @@ int fg_moe_unpermute_backward(void* d_rows, void* d_weights, const void* d_out, 
     a.rows = rows; a.ld_rows = ld_rows; a.n_rows = n_rows; a.row_of_slot = row_of_slot; a.weights = weights; a.w_dtype = w_dtype;
     a.ld_w = ld_w; a.topk = topk; a.H = H; a.d_out = d_out; a.ld_d_out = ld_d_out; a.d_rows = d_rows; a.d_w = d_weights;
     const int es = elem_size(dtype);
-    const bool vec = H % 8 == 0 && aligned16(d_out, ld_d_out * es) && (!d_weights || aligned16(rows, ld_rows * es)) && aligned16(d_rows, H * es);
+    const bool vec = aligned16(d_out, ld_d_out * es) && (!d_weights || aligned16(rows, ld_rows * es)) && aligned16(d_rows, H * es);
     return by_type(dtype, [&](auto tag) -> int {
         using E = decltype(tag);
-        FG_CUDA(vec ? fg_launch(unpermute_backward_kernel<E, 8>, (unsigned)T, threads_for(H / 8), 0, (cudaStream_t)stream, 1, a)
+        constexpr int V = 16 / sizeof(E);
+        FG_CUDA(vec ? fg_launch(unpermute_backward_kernel<E, V>, (unsigned)T, threads_for(H / V), 0, (cudaStream_t)stream, 1, a)
                     : fg_launch(unpermute_backward_kernel<E, 1>, (unsigned)T, threads_for(H), 0, (cudaStream_t)stream, 1, a));
         return FG_OK;
     });

@@ -135,6 +135,10 @@ def moe_permute(
     ``w8a8_int8_grouped_mm`` and ``scaled_grouped_mm`` take.  Differentiable in ``hidden_states``, once.
     """
     logger.debug("GEMS MOE PERMUTE")
+    if hidden_states.is_cuda:
+        done = _cabi.host.moe_permute(hidden_states, topk_ids, num_experts, scale, expert_map)
+        if done is not None:
+            return done[0], done[1], MoEPermutation(*done[2:])
     assert topk_ids.dim() == 2, "topk_ids must be [tokens, topk]"
     if topk_ids.dtype not in (torch.int32, torch.int64):
         raise NotImplementedError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
@@ -171,6 +175,10 @@ def moe_unpermute(
     read.  Returns [tokens, hidden] of the type of ``rows``.  Differentiable in ``rows`` and ``topk_weights``, once.
     """
     logger.debug("GEMS MOE UNPERMUTE")
+    if rows.is_cuda:
+        out = _cabi.host.moe_unpermute(rows, plan.row_of_slot, topk_weights)
+        if out is not None:
+            return out
     if rows.dtype not in _cabi.DTYPE_CODE:
         raise NotImplementedError(f"unsupported dtype {rows.dtype}")
     row_of_slot = plan.row_of_slot
