@@ -46,9 +46,10 @@ _SIGS = {
     "fg_silu_and_mul": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
     "fg_moe_sum": (c_int, [_P, _P, c_int64, c_int, c_int64, c_int, _P]),
     "fg_moe_sum_indexed": (c_int, [_P, _P, c_int64, c_int, c_int64, c_int, _P, _P, _P]),
+    "fg_moe_permute_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
     "fg_moe_permute": (
         c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, _P, c_int, c_int64, c_int, c_int, c_int64, c_int, c_int64, c_int64,
-                c_int64, _P]),
+                c_int64, _P, c_int64, _P]),
     "fg_moe_unpermute": (
         c_int, [_P, _P, _P, _P, c_int, c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_int, _P]),
     "fg_moe_unpermute_backward": (

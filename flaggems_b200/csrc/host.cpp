@@ -671,13 +671,15 @@ Permuted permuted(const at::Tensor& x, const at::Tensor& ids, int64_t experts, c
     p.offs = empty({experts}, ScalarType::Int, x);
     p.row_of_slot = empty({tokens, topk}, ScalarType::Int, x);
     p.slot_of_row = empty({n}, ScalarType::Int, x);
+    const int64_t need = std::max<int64_t>(fg_moe_permute_workspace_bytes(tokens, (int)topk, (int)experts), 0);
+    const at::Tensor ws = need ? empty({need}, ScalarType::Byte, x) : at::Tensor();
     throw_rc(fg_moe_permute(p.rows.data_ptr(), scale ? static_cast<float*>(p.row_scale.data_ptr()) : nullptr,
                             static_cast<int32_t*>(p.offs.data_ptr()), static_cast<int32_t*>(p.row_of_slot.data_ptr()),
                             static_cast<int32_t*>(p.slot_of_row.data_ptr()), x.data_ptr(),
                             scale ? static_cast<const float*>(scale->data_ptr()) : nullptr, ids.data_ptr(),
                             ids.scalar_type() == ScalarType::Long, map ? static_cast<const int32_t*>(map->data_ptr()) : nullptr,
                             map ? (int)map->numel() : 0, tokens, (int)topk, (int)experts, x.size(1), (int)x.element_size(),
-                            x.stride(0), cols, scale ? scale->stride(0) : 0, stream_of(x)));
+                            x.stride(0), cols, scale ? scale->stride(0) : 0, need ? ws.data_ptr() : nullptr, need, stream_of(x)));
     return p;
 }
 

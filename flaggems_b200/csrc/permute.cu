@@ -7,19 +7,14 @@
 //
 // row_of_slot holds row(t, k), or ~row for a slot without an expert: such slots own the rows behind the last
 // expert's, so that every row belongs to exactly one slot and no kernel has to look for rows that nobody names.
-#include <cooperative_groups.h>
-
 #include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace {
 
-constexpr int SORT_THREADS = 1024;
-constexpr int SORT_WARPS = SORT_THREADS / 32;
+constexpr int MAX_EXPERTS = 1024;
 
 struct SortArgs {
     const void* ids;  // [numel]
@@ -40,104 +35,74 @@ __device__ __forceinline__ int expert_of(const SortArgs& a, int64_t i) {
     return id >= 0 && id < a.num_experts ? (int)id : a.num_experts;
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+// Many slots, first launch: every CTA ranks the slots of one chunk among themselves, stable like a sort by (expert,
+// slot).  A warp owns a contiguous part of the chunk and counts it; the counts are scanned over the warps, and the
+// warp walks its part again in order.  What the row kernel needs of a chunk goes into `table`:
+//   table[e * n_chunks + c] = {slots of expert e in chunk c, slots of experts below e in chunk c}
+// The second launch turns them into the first row of every expert and chunk (the first numbers of the chunks before, and
+// the second numbers of all chunks); a slot's row is that plus its rank.  One cluster of eight CTAs, with the scans through
+// distributed shared memory, took 13 us for 65536 slots where the two launches take 6; without the second launch, every
+// token's CTA adding up its slots' rows, the row kernel takes 94 us instead of 88.  Bucket num_experts holds the
+// slots without an expert.
+constexpr int MAX_CHUNKS = 256;
+constexpr int CHUNK_THREADS = 512;
+constexpr int CHUNK_WARPS = CHUNK_THREADS / 32;
 
-// A counting sort by one cluster, stable like a sort by (expert, slot): every warp owns a contiguous segment of
-// the slots and counts it, the counts are scanned over warps, CTAs (distributed shared memory) and experts, and every warp
-// walks its segment again in order.  Bucket num_experts takes the slots without an expert.
-// SEG > 0: segments of up to 32 * SEG slots stay in registers between the two walks and are loaded all at once.
-template <int SEG>
-__global__ void __launch_bounds__(SORT_THREADS, 1) sort_slots_kernel(SortArgs a) {
+struct ChunkTable {
+    int2* table;
+    int n_chunks;
+    int chunk;  // slots, a multiple of CHUNK_THREADS
+};
+
+__global__ void __launch_bounds__(CHUNK_THREADS) rank_slots_kernel(SortArgs a, ChunkTable ct) {
     fg_pdl_wait();
     fg_pdl_trigger();
-    cg::cluster_group cluster = cg::this_cluster();
-    const int n_ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int E = a.num_experts, B = E + 1;
+    const int E = a.num_experts, B = E + 1, bits = 32 - __clz(E);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    extern __shared__ int32_t smem[];
-    int32_t* warp_hist = smem;                    // [SORT_WARPS][B] counts, then the row of the warp's next slot within the CTA
-    int32_t* cta_total = smem + SORT_WARPS * B;   // [B] read by the other CTAs
-    int32_t* base = cta_total + B;                // [B] first row of this CTA
-    __shared__ int32_t scan_tmp[SORT_WARPS];
-
-    const int64_t segments = (int64_t)n_ranks * SORT_WARPS;
-    const int64_t seg_len = ((a.numel + segments - 1) / segments + 31) / 32 * 32;
-    const int64_t seg_begin = min((rank * (int64_t)SORT_WARPS + warp) * seg_len, a.numel);
-    const int64_t seg_end = min(seg_begin + seg_len, a.numel);
-    auto bucket = [&](int64_t i) -> int { return i < seg_end ? expert_of(a, i) : -1; };
-    int kept[SEG > 0 ? SEG : 1];
-    if constexpr (SEG > 0) {
-#pragma unroll
-        for (int c = 0; c < SEG; ++c) kept[c] = bucket(seg_begin + 32 * c + lane);
-    }
-    for (int i = threadIdx.x; i < SORT_WARPS * B; i += SORT_THREADS) warp_hist[i] = 0;
+    extern __shared__ int32_t warp_hist[];  // [CHUNK_WARPS][B] counts, then the rank of the warp's next slot of the bucket
+    __shared__ int32_t scan_tmp[CHUNK_WARPS];
+    const int64_t begin = (int64_t)blockIdx.x * ct.chunk + (int64_t)warp * (ct.chunk / CHUNK_WARPS);
+    const int64_t end = min(begin + ct.chunk / CHUNK_WARPS, a.numel);
+    const int kept = begin + lane < end ? expert_of(a, begin + lane) : -1;
+    for (int i = threadIdx.x; i < CHUNK_WARPS * B; i += CHUNK_THREADS) warp_hist[i] = 0;
     __syncthreads();
-
     int32_t* my_hist = warp_hist + warp * B;
-    auto count = [&](int e) {
-        if (e >= 0) atomicAdd(&my_hist[e], 1);
-    };
-    if constexpr (SEG > 0) {
-#pragma unroll
-        for (int c = 0; c < SEG; ++c)
-            if (seg_begin + 32 * c < seg_end) count(kept[c]);
-    } else {
-        for (int64_t i0 = seg_begin; i0 < seg_end; i0 += 32) count(bucket(i0 + lane));
-    }
+    for (int64_t i = begin + lane; i < end; i += 32) atomicAdd(&my_hist[i < begin + 32 ? kept : expert_of(a, i)], 1);
     __syncthreads();
-    for (int e = threadIdx.x; e < B; e += SORT_THREADS) {
-        int32_t run = 0;
+    // over the warps per bucket, then over the buckets; B may exceed the threads
+    int32_t carry = 0;
+    for (int e0 = 0; e0 < B; e0 += CHUNK_THREADS) {
+        const int e = e0 + (int)threadIdx.x;
+        int32_t total = 0;
+        if (e < B) {
 #pragma unroll
-        for (int w = 0; w < SORT_WARPS; ++w) {
-            const int32_t t = warp_hist[w * B + e];
-            warp_hist[w * B + e] = run;
-            run += t;
+            for (int w = 0; w < CHUNK_WARPS; ++w) {
+                const int32_t n = warp_hist[w * B + e];
+                warp_hist[w * B + e] = total;
+                total += n;
+            }
         }
-        cta_total[e] = run;
-    }
-    cluster.sync();
-    const int e0 = threadIdx.x;  // num_experts <= SORT_THREADS; the last bucket follows all others and needs no scan
-    int32_t before = 0, total = 0;
-    if (e0 < E) {
-#pragma unroll 8
-        for (int r = 0; r < n_ranks; ++r) {
-            const int32_t c = cluster.map_shared_rank(cta_total, r)[e0];
-            if (r < rank) before += c;
-            total += c;
-        }
-    }
-    int32_t none_before = 0;
-    if (threadIdx.x == 0)
-        for (int r = 0; r < rank; ++r) none_before += cluster.map_shared_rank(cta_total, r)[E];
-    cluster_arrive();  // nobody leaves while the others read its counts
-    int32_t incl = total;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int32_t t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
-    }
-    if (lane == 31) scan_tmp[warp] = incl;
-    __syncthreads();
-    if (warp == 0) {
-        int32_t v = scan_tmp[lane];
+        int32_t incl = total;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int32_t t = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += t;
+            const int32_t n = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += n;
         }
-        scan_tmp[lane] = v;
+        if (lane == 31) scan_tmp[warp] = incl;
+        __syncthreads();
+        int32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < CHUNK_WARPS; ++w) {
+            if (w < warp) incl += scan_tmp[w];
+            all += scan_tmp[w];
+        }
+        if (e < B) ct.table[(int64_t)e * ct.n_chunks + blockIdx.x] = make_int2(total, carry + incl - total);
+        carry += all;
+        __syncthreads();
     }
-    __syncthreads();
-    incl += warp > 0 ? scan_tmp[warp - 1] : 0;
-    if (e0 < E) {
-        base[e0] = incl - total + before;
-        if (rank == 0) a.offs[e0] = incl;
-    }
-    if (threadIdx.x == 0) base[E] = scan_tmp[SORT_WARPS - 1] + none_before;
-    __syncthreads();
-    const int bits = 32 - __clz(E);
-    auto place = [&](int64_t i, int e) {
+    for (int64_t i0 = begin; i0 < end; i0 += 32) {
+        const int64_t i = i0 + lane;
+        const int e = i >= end ? -1 : i0 == begin ? kept : expert_of(a, i);
         // lanes of the same bucket, one vote per bit of the bucket's number (a match over 32 lanes of many different
         // buckets takes several times as long)
         unsigned peers = __ballot_sync(0xffffffffu, e >= 0);
@@ -150,20 +115,10 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) sort_slots_kernel(SortArgs a)
         if (e >= 0) {
             const unsigned below = peers & ((1u << lane) - 1u);
             if (below == 0u) my_hist[e] = cur + __popc(peers);
-            const int32_t row = base[e] + cur + __popc(below);
-            a.row_of_slot[i] = e < E ? row : ~row;
-            a.slot_of_row[row] = (int32_t)i;
+            a.row_of_slot[i] = cur + __popc(below);  // the row kernel makes it a row
         }
         __syncwarp();
-    };
-    if constexpr (SEG > 0) {
-#pragma unroll
-        for (int c = 0; c < SEG; ++c)
-            if (seg_begin + 32 * c < seg_end) place(seg_begin + 32 * c + lane, kept[c]);
-    } else {
-        for (int64_t i0 = seg_begin; i0 < seg_end; i0 += 32) place(i0 + lane, bucket(i0 + lane));
     }
-    cluster_wait();
 }
 
 // A token's row to the rows of its slots; rows of slots without an expert become zeros (their scales 1).
@@ -210,25 +165,70 @@ __device__ __forceinline__ void store_scales(const RowArgs& a, int64_t t, int k,
         a.row_scale[row * a.scale_cols + c] = r < 0 ? 1.0f : a.scale[t * a.ld_scale + c];
 }
 
-// One CTA per token: its row is read once, two pieces per thread, and written slot after slot.  Bound by the writes, which
-// are topk times the reads.  Few registers (and so many CTAs, a row each, under way) matter more than pieces per
-// thread: 8192 x 8 rows of 7168 bytes take 88 us this way, 98 with four pieces and the slots' rows in registers, 91-97 as
-// bulk copies through a ring in shared memory (6.0 TB/s of the 6.6 of a copy).
-// UNIT: the bytes of a load, 16 where everything is aligned to that.
-template <typename UNIT>
-__global__ void __launch_bounds__(256) permute_rows_kernel(RowArgs a, const int32_t* row_of_slot) {
+// Many slots, second launch, a warp per bucket: table[e, c].x becomes the first row of expert e's slots in chunk c.
+__global__ void __launch_bounds__(256) scan_chunks_kernel(SortArgs s, ChunkTable ct) {
     fg_pdl_wait();
     fg_pdl_trigger();
-    constexpr int PIECES = 2;
-    const int64_t t = blockIdx.x;
-    for (int v0 = threadIdx.x; v0 < a.units; v0 += PIECES * blockDim.x) {
-        UNIT piece[PIECES];
-        load_pieces(a, t, v0, piece);
-#pragma unroll 1
-        for (int k = 0; k < a.topk; ++k) store_pieces(a, row_of_slot[t * a.topk + k], v0, piece);
+    const int lane = threadIdx.x & 31, e = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (e > s.num_experts) return;
+    int2* of_e = ct.table + (int64_t)e * ct.n_chunks;
+    int2 v[MAX_CHUNKS / 32];
+    int32_t below = 0;
+#pragma unroll
+    for (int i = 0; i < MAX_CHUNKS / 32; ++i) {
+        const int c = 32 * i + lane;
+        v[i] = c < ct.n_chunks ? of_e[c] : make_int2(0, 0);
+        below += v[i].y;
     }
-    if (a.scale_cols)
-        for (int k = 0; k < a.topk; ++k) store_scales(a, t, k, row_of_slot[t * a.topk + k]);
+    int32_t run = __reduce_add_sync(0xffffffffu, below);
+    if (lane == 0 && e > 0) s.offs[e - 1] = run;  // the slots of the experts below e
+#pragma unroll
+    for (int i = 0; i < MAX_CHUNKS / 32; ++i) {
+        const int c = 32 * i + lane;
+        int32_t incl = v[i].x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t n = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += n;
+        }
+        if (c < ct.n_chunks) of_e[c].x = run + incl - v[i].x;
+        run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+
+// Many slots, third launch, one CTA per token: its row is read once, two pieces per thread, and written slot after
+// slot.  Bound by the writes, which are topk times the reads.  Few registers (and so many CTAs, a row each, under way)
+// matter more than pieces per thread: 8192 x 8 rows of 7168 bytes take 88 us this way, 98 with four pieces and the slots'
+// rows in registers, 91-97 as bulk copies through a ring in shared memory (6.0 TB/s of the 6.6 of a copy).
+// UNIT: the bytes of a load, 16 where everything is aligned to that.
+template <typename UNIT>
+__global__ void __launch_bounds__(256) permute_rows_kernel(SortArgs s, ChunkTable ct, RowArgs a) {
+    fg_pdl_wait();
+    fg_pdl_trigger();
+    constexpr int PIECES = 2, SLOTS = 32;
+    __shared__ int32_t row_s[SLOTS];
+    const int64_t t = blockIdx.x;
+    UNIT piece[PIECES];
+    load_pieces(a, t, threadIdx.x, piece);
+    for (int k0 = 0; k0 < a.topk; k0 += SLOTS) {
+        const int slots = min(SLOTS, a.topk - k0);
+        if ((int)threadIdx.x < slots) {
+            const int64_t slot = t * a.topk + k0 + threadIdx.x;
+            const int rank = s.row_of_slot[slot], e = expert_of(s, slot);
+            const int32_t row = ct.table[(int64_t)e * ct.n_chunks + (int)slot / ct.chunk].x + rank;
+            s.slot_of_row[row] = (int32_t)slot;
+            row_s[threadIdx.x] = s.row_of_slot[slot] = e < s.num_experts ? row : ~row;
+        }
+        __syncthreads();
+        for (int v0 = threadIdx.x; v0 < a.units; v0 += PIECES * blockDim.x) {
+            if (v0 >= PIECES * (int)blockDim.x || k0 > 0) load_pieces(a, t, v0, piece);
+#pragma unroll 1
+            for (int k = 0; k < slots; ++k) store_pieces(a, row_s[k], v0, piece);
+        }
+        if (a.scale_cols)
+            for (int k = 0; k < slots; ++k) store_scales(a, t, k, row_s[k]);
+        __syncthreads();
+    }
 }
 
 // Few slots: sorting and copying in one launch.  The CTA of a token counts for each of its slots the slots that come
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256) sort_and_permute_kernel(SortArgs s, RowAr
     fg_pdl_wait();
     fg_pdl_trigger();
     constexpr int PIECES = 4;
-    __shared__ int32_t hist[SORT_THREADS];
+    __shared__ int32_t hist[MAX_EXPERTS];
     __shared__ int32_t before[8][SLOTS_AT_ONCE];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int numel = (int)s.numel, E = s.num_experts;
@@ -530,24 +530,28 @@ bool aligned16(const void* p, int64_t stride_bytes) { return (uintptr_t)p % 16 =
 // Up to here every token's CTA looks at all slots for itself.
 constexpr int64_t ONE_LAUNCH_SLOTS = 4096;
 
-int sort_slots(const SortArgs& a, cudaStream_t st) {
-    int ranks = 1;
-    while (ranks < 8 && (int64_t)ranks * SORT_THREADS * 2 < a.numel) ranks *= 2;
-    const size_t smem = (size_t)(SORT_WARPS + 2) * (a.num_experts + 1) * sizeof(int32_t);
-    const bool kept = fg_cdiv(a.numel, (int64_t)ranks * SORT_THREADS) <= 8;
-    auto kernel = kept ? sort_slots_kernel<8> : sort_slots_kernel<0>;
+// Chunks of whole rounds of a CTA, no more than MAX_CHUNKS of them.
+ChunkTable chunk_table(void* workspace, int64_t numel) {
+    int64_t chunk = CHUNK_THREADS;
+    if (fg_cdiv(numel, chunk) > MAX_CHUNKS) chunk = fg_cdiv(fg_cdiv(numel, MAX_CHUNKS), CHUNK_THREADS) * CHUNK_THREADS;
+    return ChunkTable{reinterpret_cast<int2*>(workspace), (int)fg_cdiv(numel, chunk), (int)chunk};
+}
+
+int rank_slots(const SortArgs& a, const ChunkTable& ct, cudaStream_t st) {
+    const size_t smem = (size_t)CHUNK_WARPS * (a.num_experts + 1) * sizeof(int32_t);
     static std::mutex mu;
-    static size_t smem_set[64][2];
+    static size_t smem_set[64];
     {
         std::lock_guard<std::mutex> lock(mu);
-        size_t& have = smem_set[fg_device_index()][kept];
+        size_t& have = smem_set[fg_device_index()];
         if (have < 48 * 1024) have = 48 * 1024;
         if (smem > have) {
-            FG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            FG_CUDA(cudaFuncSetAttribute(rank_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             have = smem;
         }
     }
-    FG_CUDA(fg_launch(kernel, (unsigned)ranks, SORT_THREADS, smem, st, (unsigned)ranks, a));
+    FG_CUDA(fg_launch(rank_slots_kernel, (unsigned)ct.n_chunks, CHUNK_THREADS, smem, st, 1, a, ct));
+    FG_CUDA(fg_launch(scan_chunks_kernel, (unsigned)a.num_experts / 8 + 1, 256, 0, st, 1, a, ct));
     return FG_OK;
 }
 
@@ -555,13 +559,18 @@ int sort_slots(const SortArgs& a, cudaStream_t st) {
 
 extern "C" {
 
+int64_t fg_moe_permute_workspace_bytes(int64_t T, int topk, int num_experts) {
+    if (T < 0 || topk < 0 || num_experts <= 0 || T * topk >= (1ll << 31) - 1) return -1;
+    return T * topk <= ONE_LAUNCH_SLOTS ? 0 : (int64_t)chunk_table(nullptr, T * topk).n_chunks * (num_experts + 1) * (int64_t)sizeof(int2);
+}
+
 int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_slot, int32_t* slot_of_row, const void* x,
                    const float* scale, const void* topk_ids, int ids_are_i64, const int32_t* expert_map, int expert_map_len,
                    int64_t T, int topk, int num_experts, int64_t H, int elem_bytes, int64_t ld_x, int64_t scale_cols,
-                   int64_t ld_scale, void* stream) {
+                   int64_t ld_scale, void* workspace, int64_t workspace_bytes, void* stream) {
     FG_REQUIRE(T >= 0 && topk >= 0 && H >= 0 && scale_cols >= 0, FG_ERR_INVALID_ARGUMENT, "negative size");
-    FG_REQUIRE(num_experts > 0 && num_experts <= SORT_THREADS, FG_ERR_UNSUPPORTED, "num_experts %d must be in [1, %d]", num_experts,
-               SORT_THREADS);
+    FG_REQUIRE(num_experts > 0 && num_experts <= MAX_EXPERTS, FG_ERR_UNSUPPORTED, "num_experts %d must be in [1, %d]", num_experts,
+               MAX_EXPERTS);
     FG_REQUIRE(elem_bytes == 1 || elem_bytes == 2 || elem_bytes == 4, FG_ERR_INVALID_ARGUMENT, "elements of %d bytes", elem_bytes);
     FG_REQUIRE(T * topk < (1ll << 31) - 1 && H * elem_bytes < (1ll << 31) && scale_cols < (1ll << 31), FG_ERR_UNSUPPORTED, "size too large");
     FG_REQUIRE(expert_map == nullptr || expert_map_len > 0, FG_ERR_INVALID_ARGUMENT, "empty expert_map");
@@ -583,9 +592,17 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
         FG_CUDA(by_unit([&](auto u) { return fg_launch(sort_and_permute_kernel<decltype(u)>, (unsigned)T + 1, threads < 128 ? 128u : threads, 0, st, 1, a, r); }));
         return FG_OK;
     }
-    const int rc = sort_slots(a, st);
-    if (rc != FG_OK || numel == 0 || (H == 0 && scale_cols == 0)) return rc;
-    FG_CUDA(by_unit([&](auto u) { return fg_launch(permute_rows_kernel<decltype(u)>, (unsigned)T, threads, 0, st, 1, r, (const int32_t*)row_of_slot); }));
+    if (numel == 0) {
+        FG_CUDA(cudaMemsetAsync(offs, 0, (size_t)num_experts * sizeof(int32_t), st));
+        return FG_OK;
+    }
+    const int64_t need = fg_moe_permute_workspace_bytes(T, topk, num_experts);
+    FG_REQUIRE(workspace && (uintptr_t)workspace % 8 == 0 && workspace_bytes >= need, FG_ERR_INVALID_ARGUMENT,
+               "workspace holds %lld bytes, needs %lld (8-byte aligned)", (long long)workspace_bytes, (long long)need);
+    const ChunkTable ct = chunk_table(workspace, numel);
+    const int rc = rank_slots(a, ct, st);
+    if (rc != FG_OK) return rc;
+    FG_CUDA(by_unit([&](auto u) { return fg_launch(permute_rows_kernel<decltype(u)>, (unsigned)T, threads, 0, st, 1, a, ct, r); }));
     return FG_OK;
 }
 

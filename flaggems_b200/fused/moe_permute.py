@@ -52,12 +52,14 @@ def _permute(x, topk_ids, num_experts, scale, expert_map):
     row_of_slot = torch.empty((tokens, topk), dtype=torch.int32, device=dev)
     slot_of_row = torch.empty(n, dtype=torch.int32, device=dev)
     with _cabi.device_guard(x):
+        need = max(int(_cabi.lib().fg_moe_permute_workspace_bytes(tokens, topk, num_experts)), 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _cabi.check(_cabi.lib().fg_moe_permute(
             _cabi.ptr(rows), _cabi.ptr(row_scale), _cabi.ptr(offs), _cabi.ptr(row_of_slot), _cabi.ptr(slot_of_row),
             _cabi.ptr(x), _cabi.ptr(scale), _cabi.ptr(topk_ids), 1 if topk_ids.dtype == torch.int64 else 0,
             _cabi.ptr(expert_map), 0 if expert_map is None else expert_map.numel(), tokens, topk, num_experts, hidden,
             _ELEMENT_BYTES[x.dtype], x.stride(0), 0 if scale is None else scale.shape[1],
-            0 if scale is None else scale.stride(0), _cabi.stream_ptr(dev)))
+            0 if scale is None else scale.stride(0), _cabi.ptr(ws), need, _cabi.stream_ptr(dev)))
     return rows, row_scale, offs, row_of_slot, slot_of_row
 
 

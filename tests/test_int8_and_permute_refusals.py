@@ -126,8 +126,8 @@ def test_entry_points_check_their_sizes():
     refused(lib.fg_scaled_grouped_mm_int8(p, p, p, p, p, None, 0, p, 1025, 100, 64, 128, 128, 64, 0, p, need, None), -2, "1024 groups")
     refused(lib.fg_scaled_grouped_mm_int8(p, p, p, p, p, None, 0, p, 2, 100, 64, 131072, 131072, 64, 0, p, need, None), -2, "32 bits")
 
-    def permute(t=4, topk=2, e=4, h=8, esz=2, offs=p, rows=p, cols=0, map_=None, map_len=0):
-        return lib.fg_moe_permute(rows, None, offs, p, p, p, None, p, 0, map_, map_len, t, topk, e, h, esz, h, cols, cols, None)
+    def permute(t=4, topk=2, e=4, h=8, esz=2, offs=p, rows=p, cols=0, map_=None, map_len=0, ws=0):
+        return lib.fg_moe_permute(rows, None, offs, p, p, p, None, p, 0, map_, map_len, t, topk, e, h, esz, h, cols, cols, p, ws, None)
 
     refused(permute(e=1025), -2, "num_experts 1025")
     refused(permute(e=0), -2, "num_experts 0")
@@ -138,6 +138,11 @@ def test_entry_points_check_their_sizes():
     refused(permute(rows=None), -1, "null pointer")
     refused(permute(cols=2), -1, "null pointer")
     refused(permute(map_=p), -1, "empty expert_map")
+    for t, topk, e in ((10000, 8, 256), (1 << 20, 8, 1024), (4097, 1, 1), (1 << 27, 15, 3)):
+        need = lib.fg_moe_permute_workspace_bytes(t, topk, e)
+        assert 0 < need <= 256 * (e + 1) * 8
+        refused(permute(t=t, topk=topk, e=e, ws=need - 1), -1, "workspace holds")
+    assert lib.fg_moe_permute_workspace_bytes(512, 8, 1024) == 0 and lib.fg_moe_permute_workspace_bytes(1 << 30, 2, 8) == -1
     refused(lib.fg_moe_unpermute(p, p, p, p, 3, 4, 2, 8, 8, 8, 2, 0, None), -1, "bad weight dtype")
     refused(lib.fg_moe_unpermute(p, p, p, None, 0, 4, 2, 8, 8, 8, 2, 3, None), -1, "unsupported dtype")
     refused(lib.fg_moe_unpermute(p, p, None, None, 0, 4, 2, 8, 8, 8, 2, 0, None), -1, "null pointer")
