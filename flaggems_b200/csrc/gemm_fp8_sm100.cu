@@ -1191,14 +1191,16 @@ EncodeTiledFn get_encode_fn() {
     return fn;
 }
 
-// Byte tensor [d2][d1][d0] with d0 contiguous; box = 128 x box_rows x 1, 128-byte swizzle.
-int make_map(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1,
-             uint64_t stride2, uint32_t box_rows, int rank) {
+}  // namespace
+
+// Byte tensor [d2][d1][d0] with d0 contiguous; box = 128 x box_rows x box_d2, 128-byte swizzle.
+int fg_byte_map(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1,
+                uint64_t stride2, uint32_t box_rows, int rank, uint32_t box_d2) {
     EncodeTiledFn fn = get_encode_fn();
     FG_REQUIRE(fn != nullptr, FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     cuuint64_t dims[3] = {d0, d1, d2};
     cuuint64_t strides[2] = {stride1, stride2};
-    cuuint32_t box[3] = {128, box_rows, 1};
+    cuuint32_t box[3] = {128, box_rows, box_d2};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box,
                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1209,6 +1211,8 @@ int make_map(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_
                (unsigned long long)stride1, (unsigned long long)stride2, box_rows);
     return FG_OK;
 }
+
+namespace {
 
 // How many clusters of `slices` CTAs of the split-K kernel fit on the device at once (cached).
 template <int BN, bool BS, int OPK = 0>
@@ -1334,12 +1338,19 @@ int launch_inst(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& 
     return FG_OK;
 }
 
-int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, const void* b, int num_experts,
-                int64_t ld_b, bool block_scaled, bool fuse_silu, cudaStream_t st) {
-    FG_REQUIRE(p.K > 0 && p.K % 16 == 0, FG_ERR_UNSUPPORTED, "K = %d must be a positive multiple of 16", p.K);
+// Rows of both operands in bytes.
+int check_operands(const void* a, const void* b, int64_t K, int64_t ld_a, int64_t ld_b) {
+    FG_REQUIRE(K > 0 && K % 16 == 0, FG_ERR_UNSUPPORTED, "K = %d must be a positive multiple of 16", (int)K);
     FG_REQUIRE((uintptr_t)a % 16 == 0 && (uintptr_t)b % 16 == 0 && ld_a % 16 == 0 && ld_b % 16 == 0,
                FG_ERR_UNSUPPORTED, "a and b must be 16-byte aligned with row strides that are multiples of 16 bytes");
-    FG_REQUIRE(ld_a >= p.K && ld_b >= p.K, FG_ERR_INVALID_ARGUMENT, "row stride smaller than K");
+    FG_REQUIRE(ld_a >= K && ld_b >= K, FG_ERR_INVALID_ARGUMENT, "row stride smaller than K");
+    return FG_OK;
+}
+
+int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, const void* b, int num_experts,
+                int64_t ld_b, bool block_scaled, bool fuse_silu, cudaStream_t st) {
+    const int operands_rc = check_operands(a, b, p.K, ld_a, ld_b);
+    if (operands_rc != FG_OK) return operands_rc;
     p.status = fg_status_word_device_ptr();
     const int esz = out_elem_size(p.out_dtype);
     p.c_vec_ok = ((uintptr_t)p.c % 16 == 0) && ((p.ld_c * esz) % 16 == 0);
@@ -1404,10 +1415,10 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     if (tiles == 0) return FG_OK;
 
     CUtensorMap ta, tb;
-    int rc = make_map(&ta, a, (uint64_t)p.K, (uint64_t)a_rows, 1, (uint64_t)ld_a, 0,
+    int rc = fg_byte_map(&ta, a, (uint64_t)p.K, (uint64_t)a_rows, 1, (uint64_t)ld_a, 0,
                       (uint32_t)(p.gather_div > 0 && !p.a_contiguous ? 1 : pair ? BLOCK_M : p.grouped ? p.block_rows : p.a_box_rows), 2);
     if (rc != FG_OK) return rc;
-    rc = make_map(&tb, b, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)num_experts, (uint64_t)ld_b,
+    rc = fg_byte_map(&tb, b, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)num_experts, (uint64_t)ld_b,
                   (uint64_t)ld_b * (uint64_t)p.N, (uint32_t)((fuse_silu || pair) ? bn / 2 : bn), 3);
     if (rc != FG_OK) return rc;
     if (pair) {
@@ -1497,6 +1508,9 @@ __global__ void bounded_wait_selftest_kernel(unsigned int* status, uint64_t limi
     }
 }
 
+// Up to here int8 products are int8_skinny.cu's.
+constexpr int64_t INT8_SKINNY_M = 32;
+
 // Dense product of e4m3 (operand 0) or int8 (1) operands.
 int scaled_mm_common(int operand, void* c, const void* a, const void* b, const float* sa, const float* sb, const void* bias,
                      int bias_dtype, int64_t M, int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c, int sa_mode,
@@ -1517,6 +1531,12 @@ int scaled_mm_common(int operand, void* c, const void* a, const void* b, const f
     p.bias_dtype = bias_dtype;
     p.block_rows = BLOCK_M;
     p.int8 = operand;
+    if (operand == 1 && M <= INT8_SKINNY_M) {
+        const int rc = check_operands(a, b, K, ld_a, ld_b);
+        if (rc != FG_OK) return rc;
+        return fg_int8_skinny(FgSkinny{c, (const int8_t*)a, (const int8_t*)b, sa, sb, bias, M, N, K, ld_a, ld_b, ld_c, sa_mode, sb_mode,
+                                       out_dtype, bias_dtype, bias_after_round}, (cudaStream_t)stream);
+    }
     return launch_gemm(p, a, M, ld_a, b, 1, ld_b, false, false, (cudaStream_t)stream);
 }
 

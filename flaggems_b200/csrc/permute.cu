@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(256) sort_and_permute_kernel(SortArgs s, RowAr
     load_pieces(a, t, v0, piece);
     for (int k0 = 0; k0 < a.topk; k0 += SLOTS_AT_ONCE) {
         const int first = (int)t * a.topk + k0;
-        // (expert, slot) as one number: fits because numel * (num_experts + 1) < 2^31 here
+        // (expert, slot) as one number: below 65536 * 1025
         int32_t key[SLOTS_AT_ONCE], n[SLOTS_AT_ONCE];
 #pragma unroll
         for (int k = 0; k < SLOTS_AT_ONCE; ++k) {
@@ -527,8 +527,15 @@ unsigned threads_for(int64_t n) { return n >= 256 ? 256u : (unsigned)(n < 32 ? 3
 
 bool aligned16(const void* p, int64_t stride_bytes) { return (uintptr_t)p % 16 == 0 && stride_bytes % 16 == 0; }
 
-// Up to here every token's CTA looks at all slots for itself.
-constexpr int64_t ONE_LAUNCH_SLOTS = 4096;
+// Whether every token's CTA looks at all slots for itself, one launch instead of three.  What that costs grows with
+// tokens x slots and hides behind the rows that are copied meanwhile.  Measured, one launch against three: 8 experts per
+// token and rows of 14 KB, 2048 slots 8.8 / 12.7 us, 4096 slots 16.0 / 17.6, 6144 slots 28.9 / 24.6; 2 and 8 KB: 1024 slots 6.6 /
+// 6.8, 2048 slots 12.7 / 8.2; 8 and 1 KB: 512 slots 6.1 / 6.5, 2048 slots 9.2 / 6.8.
+constexpr int64_t ONE_LAUNCH_LOOKS = 65536;
+bool one_launch(int64_t T, int64_t numel, int64_t row_bytes) {
+    const int64_t most = 64 * row_bytes > ONE_LAUNCH_LOOKS ? 64 * row_bytes : ONE_LAUNCH_LOOKS;
+    return numel <= 65536 && T * numel <= most;
+}
 
 // Chunks of whole rounds of a CTA, no more than MAX_CHUNKS of them.
 ChunkTable chunk_table(void* workspace, int64_t numel) {
@@ -561,7 +568,7 @@ extern "C" {
 
 int64_t fg_moe_permute_workspace_bytes(int64_t T, int topk, int num_experts) {
     if (T < 0 || topk < 0 || num_experts <= 0 || T * topk >= (1ll << 31) - 1) return -1;
-    return T * topk <= ONE_LAUNCH_SLOTS ? 0 : (int64_t)chunk_table(nullptr, T * topk).n_chunks * (num_experts + 1) * (int64_t)sizeof(int2);
+    return one_launch(T, T * topk, 0) ? 0 : (int64_t)chunk_table(nullptr, T * topk).n_chunks * (num_experts + 1) * (int64_t)sizeof(int2);
 }
 
 int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_slot, int32_t* slot_of_row, const void* x,
@@ -588,7 +595,7 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
     auto by_unit = [&](auto&& go) -> cudaError_t {
         return vec ? go(uint4()) : elem_bytes == 4 ? go((unsigned int)0) : elem_bytes == 2 ? go((unsigned short)0) : go((unsigned char)0);
     };
-    if (numel > 0 && numel <= ONE_LAUNCH_SLOTS) {
+    if (numel > 0 && one_launch(T, numel, row_bytes)) {
         FG_CUDA(by_unit([&](auto u) { return fg_launch(sort_and_permute_kernel<decltype(u)>, (unsigned)T + 1, threads < 128 ? 128u : threads, 0, st, 1, a, r); }));
         return FG_OK;
     }

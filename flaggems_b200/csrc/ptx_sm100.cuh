@@ -5,6 +5,10 @@
 #include <cuda.h>
 #include <stdint.h>
 
+// Tensor map of bytes [d2][d1][d0] with d0 contiguous (rank 2: d2 is 1); box = 128 x box_rows x box_d2, 128-byte swizzle.
+int fg_byte_map(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1, uint64_t stride2,
+                uint32_t box_rows, int rank, uint32_t box_d2 = 1);
+
 namespace fgptx {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

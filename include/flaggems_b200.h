@@ -208,7 +208,7 @@ int fg_moe_sum_indexed(const void* in, void* out, int64_t M, int topk, int64_t K
  *   rows[r]               x[t] (elem_bytes 1, 2 or 4 per value, row stride ld_x elements); zeros without an expert
  *   row_scale[r]          scale[t] (scale_cols values, row stride ld_scale; scale_cols may be 0); ones without an expert
  * rows and row_scale are contiguous.  At most 1024 experts, T * topk < 2^31 - 1.  Scratch is the caller's workspace of
- * fg_moe_permute_workspace_bytes(T, topk, num_experts) bytes, 8-byte aligned (0 bytes, and NULL, for few slots). */
+ * fg_moe_permute_workspace_bytes(T, topk, num_experts) bytes, 8-byte aligned (0 for few slots: then it may be NULL). */
 int64_t fg_moe_permute_workspace_bytes(int64_t T, int topk, int num_experts);
 int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_slot, int32_t* slot_of_row, const void* x,
                    const float* scale, const void* topk_ids, int ids_are_i64, const int32_t* expert_map, int expert_map_len,

@@ -142,7 +142,7 @@ def test_entry_points_check_their_sizes():
         need = lib.fg_moe_permute_workspace_bytes(t, topk, e)
         assert 0 < need <= 256 * (e + 1) * 8
         refused(permute(t=t, topk=topk, e=e, ws=need - 1), -1, "workspace holds")
-    assert lib.fg_moe_permute_workspace_bytes(512, 8, 1024) == 0 and lib.fg_moe_permute_workspace_bytes(1 << 30, 2, 8) == -1
+    assert lib.fg_moe_permute_workspace_bytes(64, 8, 1024) == 0 and lib.fg_moe_permute_workspace_bytes(1 << 30, 2, 8) == -1
     refused(lib.fg_moe_unpermute(p, p, p, p, 3, 4, 2, 8, 8, 8, 2, 0, None), -1, "bad weight dtype")
     refused(lib.fg_moe_unpermute(p, p, p, None, 0, 4, 2, 8, 8, 8, 2, 3, None), -1, "unsupported dtype")
     refused(lib.fg_moe_unpermute(p, p, None, None, 0, 4, 2, 8, 8, 8, 2, 0, None), -1, "null pointer")
