@@ -79,6 +79,12 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
     const int w_block = a.rows * BLOCK_K, w_bytes = KB * w_block, stage_bytes = w_bytes + KB * TOKENS * BLOCK_K;
     int* sums = reinterpret_cast<int*>(ring + (size_t)a.stages * stage_bytes);  // [TOKENS][rows]
     volatile uint32_t* abort_flag = &abort_word;
+    const int steps = ((int)p.K + KB * BLOCK_K - 1) / (KB * BLOCK_K);  // stages per group
+    if (warp == WARPS && lane == 0) {
+        // While the kernel before this one drains, the first stages of the weight come as far as L2.
+        if (a.wide)
+            for (int step = 0; step < min(a.stages, steps); ++step) tma_prefetch_3d(&tm_w, 0, blockIdx.x * a.rows, step * KB);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
             mbar_init(&full_bar[s], 1);
@@ -92,7 +98,6 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
     for (int i = threadIdx.x; i < TOKENS * a.rows; i += THREADS) sums[i] = 0;
     __syncthreads();
     fg_pdl_wait();
-    const int steps = ((int)p.K + KB * BLOCK_K - 1) / (KB * BLOCK_K);  // stages per group
 
     if (warp == WARPS) {
         if (lane == 0) {
