@@ -80,7 +80,7 @@ struct FgGroupedGemm {
 };
 int fg_grouped_gemm(const FgGroupedGemm& g, cudaStream_t stream);
 
-// c[m, n] of up to 32 int8 tokens a [M, K] and an int8 weight b [N, K]: the arguments of fg_scaled_mm_int8, checked.
+// c[m, n] of few int8 tokens a [M, K] and an int8 weight b [N, K]: the arguments of fg_scaled_mm_int8, checked.
 struct FgSkinny {
     void* c;
     const int8_t *a, *b;
@@ -89,6 +89,7 @@ struct FgSkinny {
     int64_t M, N, K, ld_a, ld_b, ld_c;
     int sa_mode, sb_mode, out_dtype, bias_dtype, bias_after_round;
 };
+bool fg_int8_is_skinny(int64_t M, int64_t N);
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st);
 
 // The rows of a grouped product's result that follow its last group, to be filled with zeros (c NULL: left as they are).

@@ -84,6 +84,7 @@ struct GemmParams {
     const int32_t* num_post_pad;
     int block_rows;  // grouped: rows per m-tile (TMA box rows of A), <= 128; CTA pairs: 256, each CTA fetches its 128
     int a_box_rows;  // dense: TMA box rows of A (128, or fewer when M is small)
+    int tile_n;      // int8: columns of a tile, a multiple of 32 up to BN
     int64_t numel;
     // Grouped, gather_div > 0: A (and its per-row scales) holds one row per token and route slot s reads
     // row s / gather_div through sorted_ids; gather_div == 0: rows of A are already in sorted order.
@@ -306,7 +307,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     static_assert(!ASTORE || (BLOCK_SCALED && !SPLITK), "the store warp serves the block-scaled tiles");
     constexpr bool INT8 = OPK == 1;
     static_assert(OPK == 0 || !BLOCK_SCALED, "block scales are for e4m3 operands");
-    static_assert(OPK < 2 || (!SPLITK && !SMALL_A), "16-bit operands serve the grouped tiles");
+    static_assert(OPK == 0 || !SMALL_A, "int8 products of so few rows are int8_skinny.cu's");
+    static_assert(OPK < 2 || !SPLITK, "16-bit operands serve the grouped tiles");
     // accumulator word -> fp32
     auto acc_f = [](uint32_t raw) -> float {
         if constexpr (INT8) return __int2float_rn((int)raw);
@@ -316,7 +318,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     static_assert(!PAIR || (!SPLITK && !BLOCK_SCALED && !SMALL_A), "the CTA pair serves the tiles without block scales");
     static_assert(!FUSE_SILU || BN >= 128, "fused SiLU needs a tile of at least 128 columns");
     constexpr int STAGES = C::STAGES;
-    constexpr int OUT_TILE_N = FUSE_SILU ? BN / 2 : BN;  // output columns per tile
+    // Output columns per tile.  int8 tiles may be narrower than BN, so that their number fits the SMs.
+    constexpr bool ANY_WIDTH = INT8 && !FUSE_SILU && !SPLITK && BN >= 128;
+    constexpr int FULL_TILE_N = FUSE_SILU ? BN / 2 : BN;
+    const int OUT_TILE_N = ANY_WIDTH ? p.tile_n : FULL_TILE_N;
     // DUAL (block-scaled wide tiles): warps 1 and 2 issue the MMAs of alternate K blocks.  A K block's
     // trip through the issuing warp (two barrier waits of ~100 cycles each even when they are already
     // complete, four MMAs at ~46 cycles of issue each, two commits) measured ~530 cycles, more than
@@ -412,7 +417,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         tile_first = blockIdx.x / k_slices;
         tile_step = gridDim.x / k_slices;
     }
-    const uint32_t stage_tx = (uint32_t)((PAIR ? BLOCK_M : p.grouped ? p.block_rows : p.a_box_rows) * BLOCK_K + C::B_BYTES);
+    const uint32_t b_tx = ANY_WIDTH ? (uint32_t)((PAIR ? OUT_TILE_N / 2 : OUT_TILE_N) * BLOCK_K) : (uint32_t)C::B_BYTES;
+    const uint32_t stage_tx = (uint32_t)((PAIR ? BLOCK_M : p.grouped ? p.block_rows : p.a_box_rows) * BLOCK_K) + b_tx;
 
     if (warp < C::FIRST_EPI_WARP) {
       if constexpr (C::REBALANCE_REGS) setmaxnreg_dec<C::REGS_PRODUCER>();
@@ -447,7 +453,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                         return real ? s / p.gather_div : 0;
                     };
                     rows = make_int4(token(sid.x), token(sid.y), token(sid.z), token(sid.w));
-                    tx = (uint32_t)(__popc(__ballot_sync(0xffffffffu, mine)) * 4 * BLOCK_K + C::B_BYTES);
+                    tx = (uint32_t)(__popc(__ballot_sync(0xffffffffu, mine)) * 4 * BLOCK_K) + b_tx;
                 }
                 for (int kb = kb_begin; kb < kb_end; ++kb) {
                     FG_PROF_T0(tw);
@@ -465,7 +471,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                         if (cta_rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2u * stage_tx);
                         tma_load_2d_2cta(sa, &tm_a, bar0, kb * BLOCK_K, m0);
                         // this CTA's 128 of the 256 rows of B; fused SiLU: gate rows here, up rows in the odd CTA
-                        tma_load_3d_2cta(sb, &tm_b, bar0, kb * BLOCK_K, n0 + (int)cta_rank * (FUSE_SILU ? p.N / 2 : BN / 2), expert);
+                        tma_load_3d_2cta(sb, &tm_b, bar0, kb * BLOCK_K, n0 + (int)cta_rank * (FUSE_SILU ? p.N / 2 : OUT_TILE_N / 2), expert);
                         if (++stage == STAGES) {
                             stage = 0;
                             phase ^= 1u;
@@ -506,7 +512,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         // ------------------------------- store warp -----------------------------------------
         // Writes parked tiles out: one 16-byte piece per lane, a whole row (or two) per instruction,
         // to the row's own destination (plain, scattered or on a peer GPU).
-        constexpr int ROW_BYTES = OUT_TILE_N * 2;
+        constexpr int ROW_BYTES = FULL_TILE_N * 2;
         constexpr int LANES_PER_ROW = ROW_BYTES / 16;      // 32 or 16
         constexpr int ROWS_PER_STEP = 32 / LANES_PER_ROW;  // 1 or 2
         uint32_t it = 0;
@@ -618,7 +624,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         // before the current block's MMAs are issued, and the blocking wait is only the fallback.
         if (cta_rank == 0) {
             constexpr int MMA_M = PAIR ? 2 * BLOCK_M : BLOCK_M;
-            constexpr uint32_t idesc = OPK == 1 ? umma_idesc_s8_s32(MMA_M, BN)
+            const uint32_t idesc = OPK == 1 ? umma_idesc_s8_s32(MMA_M, ANY_WIDTH ? OUT_TILE_N : BN)
                                        : OPK >= 2 ? umma_idesc_16bit_f32(MMA_M, BN, OPK == 2)
                                                   : umma_idesc_e4m3_f32(MMA_M, BN);
             int stage = 0;
@@ -784,6 +790,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 #pragma unroll
                     for (int c = 0; c < OUT_CHUNKS; ++c) {
                         const int col = out_col_base + 32 * c;
+                        if (ANY_WIDTH && col >= n0 + OUT_TILE_N) break;
                         const int nc = min(32, p.n_out - col);
                         if (nc > 0) store_chunk(out_ptr, col, z, nc, p.out_dtype, p.c_vec_ok);
                     }
@@ -826,6 +833,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 #pragma unroll
                 for (int c = 0; c < OUT_CHUNKS; ++c) {
                     const int col = out_col_base + 32 * c;
+                    if (ANY_WIDTH && col >= n0 + OUT_TILE_N) break;
                     uint32_t raw[32];
                     float v[32];
                     if constexpr (FUSE_SILU) {
@@ -1027,7 +1035,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     // at once and the row the store warp reads at once both spread over all banks.
                     ok = mbar_wait(park_free, (park_iter & 1u) ^ 1u, abort_flag, p.status, 7);
                     if (!ok) break;
-                    constexpr int ROW_BYTES = OUT_TILE_N * 2;
+                    constexpr int ROW_BYTES = FULL_TILE_N * 2;
                     uint8_t* prow = park_tile + r_in_tile * ROW_BYTES;
 #pragma unroll
                     for (int c = 0; c < OUT_CHUNKS; ++c) {
@@ -1303,7 +1311,8 @@ int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& 
         max_clusters = n < fg_num_sms() / 2 ? n : fg_num_sms() / 2;
     }
     const int clusters = pair_tiles < max_clusters ? pair_tiles : max_clusters;
-    FG_CUDA(fg_launch_when(false, kernel, (unsigned)(2 * clusters), C::THREADS, C::SMEM_BYTES, st, 2, ta, tb, p));
+    // int8 products: early where they are short, as the single-CTA kernels; the other kinds keep their launches.
+    FG_CUDA(fg_launch_when(OPK == 1 && !p.grouped && short_run(2 * (int64_t)pair_tiles), kernel, (unsigned)(2 * clusters), C::THREADS, C::SMEM_BYTES, st, 2, ta, tb, p));
     return FG_OK;
 }
 
@@ -1337,6 +1346,39 @@ int launch_inst(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& 
     FG_CUDA(fg_launch_when(short_run(max_tiles), kernel, (unsigned)grid, C::THREADS, C::SMEM_BYTES, st, 1, ta, tb, p));
     return FG_OK;
 }
+
+// Tile of a dense int8 product: the width and the kind (one CTA per 128 rows, or a CTA pair per 256) with the least estimated time,
+// which is the number of waves of tiles times what a block of K takes, which hardly depends on the width below 256
+// (the ring's round trip; above, the 64 bytes per cycle that an SM takes in).  So a narrower tile pays where it saves a
+// wave, and a pair where a tile's K is long enough for its dearer start.  The constants (ns) are fitted to 5 weights x 12 row counts
+// x 11 tiles on this chip, and the choices are within 5 % of the best of the 11.  Measured, 256-wide single / 256-wide pair / this:
+// 1037 x 6144 x 4096 32.3 / 28.7 / 27.0 us (pairs of 224 columns, two full waves), 300 x 7168 x 2048 13.3 / 13.2 / 12.0 (single,
+// 160), 777 x 4096 x 14336 51.1 / 44.1 / 44.1, 1037 x 4096 x 14336 52.3 / 75.0 / 52.3, 128 x 6144 x 4096 18.9 / 17.2 / 15.1 (single, 96).
+struct Int8Tile {
+    bool pair;
+    int width;
+};
+Int8Tile int8_tile(int64_t M, int64_t N, int64_t k_blocks, int sms) {
+    Int8Tile best{false, 256};
+    int64_t least = INT64_MAX;
+    auto offer = [&](bool pair, int width, int64_t start, int64_t per_block) {
+        const int64_t tiles = fg_cdiv(M, pair ? 2 * BLOCK_M : BLOCK_M) * fg_cdiv(N, width);
+        const int64_t time = start + fg_cdiv(tiles, pair ? sms / 2 : sms) * k_blocks * per_block;
+        if (time < least) {
+            least = time;
+            best = Int8Tile{pair, width};
+        }
+    };
+    for (int width = 256; width >= 96; width -= 32) offer(false, width, 4000, 290 + 130 * width / 256);
+    offer(false, 64, 4000, 285);
+    if (M > BLOCK_M)
+        for (int width = 256; width >= 128; width -= 32) offer(true, width, 5500, 265 + 80 * width / 256);
+    return best;
+}
+// Up to 128 rows and up to here in K the tiles above beat split K, whose reduction through the cluster costs about as much
+// as 40 blocks: 128 x 6144 x 4096 15.1 / 20.8 us, 128 x 7168 x 2048 10.0 / 18.7, but 128 x 2112 x 7168 21.0 / 17.6 and
+// 128 x 4096 x 14336 36.6 / 30.0.
+constexpr int SPLITK_MIN_K_INT8 = 5120;
 
 // Rows of both operands in bytes.
 int check_operands(const void* a, const void* b, int64_t K, int64_t ld_a, int64_t ld_b) {
@@ -1406,11 +1448,21 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     // Large dense products: a pair of CTAs per 256 x 256 tile (a third less L2 and shared-memory
     // traffic per flop: +4-5 % under the power cap) once there are at least three waves of such
     // tiles; with fewer, the coarser tiles lose more to the ragged last wave than they gain.
-    const int64_t pair_tiles = fg_cdiv(p.M, 2 * BLOCK_M) * fg_cdiv(p.n_out, fuse_silu ? 128 : 256);
-    const bool pair = grouped_pair || (!p.grouped && !fuse_silu && !block_scaled && bn == 256 && k_slices == 1 &&
+    p.tile_n = fuse_silu ? bn / 2 : bn;
+    bool int8_pair = false;
+    if (p.int8 == 1 && !p.grouped) {
+        if (k_slices > 1 && p.K <= SPLITK_MIN_K_INT8) k_slices = 1;
+        if (k_slices == 1) {
+            const Int8Tile t = int8_tile(p.M, p.n_out, fg_cdiv(p.K, BLOCK_K), sms);
+            int8_pair = t.pair;
+            p.tile_n = t.width;
+            bn = t.width > 128 || t.pair ? 256 : t.width > 64 ? 128 : 64;
+        }
+    }
+    const int64_t pair_tiles = fg_cdiv(p.M, 2 * BLOCK_M) * fg_cdiv(p.n_out, fuse_silu ? 128 : int8_pair ? p.tile_n : 256);
+    const bool pair = int8_pair || grouped_pair || (p.int8 == 0 && !p.grouped && !fuse_silu && !block_scaled && bn == 256 && k_slices == 1 &&
                                        pair_tiles >= 3 * (int64_t)(sms / 2) && pair_tiles < (1ll << 30) && pair_enabled());
-    const int out_tile = fuse_silu ? bn / 2 : bn;
-    const int64_t tiles = m_tiles * fg_cdiv(p.n_out, out_tile);
+    const int64_t tiles = m_tiles * fg_cdiv(p.n_out, p.tile_n);
     FG_REQUIRE(tiles < (1ll << 31), FG_ERR_UNSUPPORTED, "too many tiles");
     if (tiles == 0) return FG_OK;
 
@@ -1419,7 +1471,7 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
                       (uint32_t)(p.gather_div > 0 && !p.a_contiguous ? 1 : pair ? BLOCK_M : p.grouped ? p.block_rows : p.a_box_rows), 2);
     if (rc != FG_OK) return rc;
     rc = fg_byte_map(&tb, b, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)num_experts, (uint64_t)ld_b,
-                  (uint64_t)ld_b * (uint64_t)p.N, (uint32_t)((fuse_silu || pair) ? bn / 2 : bn), 3);
+                  (uint64_t)ld_b * (uint64_t)p.N, (uint32_t)(fuse_silu ? bn / 2 : pair ? p.tile_n / 2 : p.tile_n), 3);
     if (rc != FG_OK) return rc;
     if (pair) {
         FG_REQUIRE(pair_tiles < (1ll << 30), FG_ERR_UNSUPPORTED, "too many tiles");
@@ -1443,8 +1495,6 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
             if (k_slices > 1) return bn == 256 ? launch_splitk<256, false, 1>(ta, tb, p, t, k_slices, st)
                                                : launch_splitk<128, false, 1>(ta, tb, p, t, k_slices, st);
             if (bn == 64) return launch_inst<64, false, false, false, false, 1>(ta, tb, p, t, st);
-            if (small_a) return launch_inst<32, false, false, true, false, 1>(ta, tb, p, t, st);
-            if (bn == 32) return launch_inst<32, false, false, false, false, 1>(ta, tb, p, t, st);
         }
         auto by_kind = [&](auto bn_tag, auto silu_tag) -> int {
             constexpr int B = decltype(bn_tag)::value;
@@ -1508,9 +1558,6 @@ __global__ void bounded_wait_selftest_kernel(unsigned int* status, uint64_t limi
     }
 }
 
-// Up to here int8 products are int8_skinny.cu's.
-constexpr int64_t INT8_SKINNY_M = 32;
-
 // Dense product of e4m3 (operand 0) or int8 (1) operands.
 int scaled_mm_common(int operand, void* c, const void* a, const void* b, const float* sa, const float* sb, const void* bias,
                      int bias_dtype, int64_t M, int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c, int sa_mode,
@@ -1531,7 +1578,7 @@ int scaled_mm_common(int operand, void* c, const void* a, const void* b, const f
     p.bias_dtype = bias_dtype;
     p.block_rows = BLOCK_M;
     p.int8 = operand;
-    if (operand == 1 && M <= INT8_SKINNY_M) {
+    if (operand == 1 && fg_int8_is_skinny(M, N)) {
         const int rc = check_operands(a, b, K, ld_a, ld_b);
         if (rc != FG_OK) return rc;
         return fg_int8_skinny(FgSkinny{c, (const int8_t*)a, (const int8_t*)b, sa, sb, bias, M, N, K, ld_a, ld_b, ld_c, sa_mode, sb_mode,

@@ -1,6 +1,6 @@
 // Products of few int8 tokens and a large int8 weight: C[m, n] = sum_k A[m, k] B[n, k], scaled per token and channel.
 //
-// With up to 32 tokens the weight's bytes are all the work, and the job is to keep enough of them under way on every
+// With so few tokens the weight's bytes are all the work, and the job is to keep enough of them under way on every
 // SM, from the first cycle to the last.  A CTA owns groups of weight rows, as many per group as it takes for the groups to
 // cover the SMs once (or a whole number of times); one thread streams them by TMA into a ring that fills the shared
 // memory, across the ends of groups, so that no epilogue interrupts the stream.  Eight warps multiply with mma.m16n8k32
@@ -26,7 +26,7 @@ constexpr int THREADS = 32 * (WARPS + 1);
 constexpr int BLOCK_K = 128;
 constexpr int MAX_ROWS = 256;
 constexpr int MAX_STAGES = 16;
-constexpr int RING_BYTES = 190 * 1024;
+constexpr int SMEM_BYTES = 224 * 1024;  // ring, sums and alignment
 
 struct StreamArgs {
     FgSkinny p;
@@ -230,14 +230,15 @@ int launch(StreamArgs& a, cudaStream_t st) {
         std::lock_guard<std::mutex> lock(mu);
         bool& done = attr_done[fg_device_index()];
         if (!done) {
-            FG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES + 33 * 1024 + 1024));
+            FG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
             done = true;
         }
     }
     const int grid = a.groups < fg_num_sms() ? a.groups : fg_num_sms();
     const int64_t stage = (int64_t)KB * (a.rows + 8 * NT) * BLOCK_K;
     const int64_t all = fg_cdiv(p.K, KB * BLOCK_K) * fg_cdiv(a.groups, grid);
-    int64_t stages = RING_BYTES / stage;
+    const int64_t sums = (int64_t)8 * NT * a.rows * sizeof(int) + 1024;
+    int64_t stages = (SMEM_BYTES - sums) / stage;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
     if (stages > all) stages = all;
     FG_REQUIRE(stages >= 1, FG_ERR_UNSUPPORTED, "a stage of %lld bytes does not fit", (long long)stage);
@@ -254,7 +255,7 @@ int launch(StreamArgs& a, cudaStream_t st) {
         if (rc == FG_OK) rc = fg_byte_map(&tm_x, p.a, (uint64_t)p.K, (uint64_t)p.M, 1, (uint64_t)p.ld_a, (uint64_t)p.ld_a * p.M, 8 * NT, 3);
     }
     if (rc != FG_OK) return rc;
-    const size_t smem = (size_t)(stages * stage) + (size_t)8 * NT * a.rows * sizeof(int) + 1024;
+    const size_t smem = (size_t)(stages * stage + sums);
     FG_CUDA(fg_launch(kernel, (unsigned)grid, THREADS, smem, st, 1, tm_w, tm_x, a));
     return FG_OK;
 }
@@ -265,20 +266,36 @@ int launch_rows(StreamArgs& a, cudaStream_t st) {
     if (a.rows <= 16) return launch<NT, 1, 8>(a, st);
     if (a.rows <= 32) return launch<NT, 2, 8>(a, st);
     if (a.rows <= 64) return launch<NT, 2, 4>(a, st);
-    if (a.rows <= 128) return launch<NT, 2, 2>(a, st);
-    return launch<NT, 2, 1>(a, st);
+    if constexpr (NT < 8) {
+        if (a.rows <= 128) return launch<NT, 2, 2>(a, st);
+        return launch<NT, 2, 1>(a, st);
+    }
+    fg_set_error("groups of %d rows are built for up to 32 tokens", a.rows);
+    return FG_ERR_UNSUPPORTED;
+}
+
+// Rows per group, as many groups as that gives: as few rounds of groups as their height allows, and in those all
+// groups of one height.
+int group_rows(int64_t N) {
+    const int64_t rounds = fg_cdiv(N, (int64_t)MAX_ROWS * fg_num_sms());
+    return (int)(fg_cdiv(fg_cdiv(N, rounds * fg_num_sms()), 16) * 16);
 }
 
 }  // namespace
 
+// Up to 32 tokens the weight streams at the rate of HBM (6.5 TB/s between a 117 MB and a 176 MB weight, and 4 us around
+// that); above, mma.sync runs out (0.4 PFLOP/s): with groups of up to 64 rows, where the tiles of tcgen05 are
+// slower still, up to 64 tokens.  Measured, this against the tcgen05 tiles: M = 1, N x K = 6144 x 4096 6.3 / 11.0 us, 28672 x 4096
+// 21.4 / 25.5, 24576 x 7168 31.0 / 36.8; M = 32 9.4 / 13.4, 25.2 / 26.5, 37.6 / 37.9; M = 64 14.7 / 15.9, 38.8 / 27.1,
+// 56.0 / 38.8.
+bool fg_int8_is_skinny(int64_t M, int64_t N) { return M <= 32 || (M <= 64 && group_rows(N) <= 64); }
+
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st) {
-    FG_REQUIRE(p.M > 0 && p.M <= 32 && p.N > 0 && p.K > 0 && p.K % 16 == 0, FG_ERR_UNSUPPORTED, "bad sizes");
+    FG_REQUIRE(p.M > 0 && p.N > 0 && fg_int8_is_skinny(p.M, p.N) && p.K > 0 && p.K % 16 == 0, FG_ERR_UNSUPPORTED, "bad sizes");
     StreamArgs a{};
     a.p = p;
     a.status = fg_status_word_device_ptr();
-    // As few rounds of groups as their height allows, and in those all groups of one height.
-    const int64_t rounds = fg_cdiv(p.N, (int64_t)MAX_ROWS * fg_num_sms());
-    a.rows = (int)(fg_cdiv(fg_cdiv(p.N, rounds * fg_num_sms()), 16) * 16);
+    a.rows = group_rows(p.N);
     a.groups = (int)fg_cdiv(p.N, a.rows);
-    return p.M <= 8 ? launch_rows<1>(a, st) : p.M <= 16 ? launch_rows<2>(a, st) : launch_rows<4>(a, st);
+    return p.M <= 8 ? launch_rows<1>(a, st) : p.M <= 16 ? launch_rows<2>(a, st) : p.M <= 32 ? launch_rows<4>(a, st) : launch_rows<8>(a, st);
 }
