@@ -858,12 +858,25 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                         tmem_ld_32x32b_x32(tbuf + 128 * half + 32 * c, raw);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = col_scale[32 * c + i] * (sa * acc_f(raw[i])) * weight;
+                        for (int q = 0; q < 8; ++q) {
+                            const float4 s = reinterpret_cast<const float4*>(col_scale + 32 * c)[q];
+                            v[4 * q] = s.x * (sa * acc_f(raw[4 * q])) * weight;
+                            v[4 * q + 1] = s.y * (sa * acc_f(raw[4 * q + 1])) * weight;
+                            v[4 * q + 2] = s.z * (sa * acc_f(raw[4 * q + 2])) * weight;
+                            v[4 * q + 3] = s.w * (sa * acc_f(raw[4 * q + 3])) * weight;
+                        }
                         if (p.bias) {
+                            if (p.bias_after_round) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float b = col_bias[32 * c + i];
-                                v[i] = p.bias_after_round ? round_through(v[i], p.out_dtype) + b : v[i] + b;
+                                for (int i = 0; i < 32; ++i) v[i] = round_through(v[i], p.out_dtype);
+                            }
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                const float4 b = reinterpret_cast<const float4*>(col_bias + 32 * c)[q];
+                                v[4 * q] += b.x;
+                                v[4 * q + 1] += b.y;
+                                v[4 * q + 2] += b.z;
+                                v[4 * q + 3] += b.w;
                             }
                         }
                     }
