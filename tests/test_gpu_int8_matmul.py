@@ -44,16 +44,64 @@ def _check(got, pre, bias=None, rounded_before_bias=False):
     assert bool((err <= bound * 1.001).all()), (float(err.max()), float((err / bound.clamp_min(1e-300)).max()))
 
 
-# one row block of every tile width, split K, the narrow tiles, ragged edges in every dimension, the CTA pair
-SHAPES = [(1, 1, 16), (1, 256, 128), (1, 6144, 4096), (1, 2112, 7168), (2, 33, 48), (7, 130, 2064), (16, 28672, 4096), (31, 4096, 4096),
-          (32, 300, 16), (33, 208, 496), (64, 24576, 1040), (83, 7744, 3888), (128, 4096, 14336), (129, 144, 144), (130, 4097, 528),
-          (257, 9500, 256), (1024, 6144, 4096), (1037, 6145, 4096), (4099, 8191, 512), (8192, 8192, 1024)]
+# few tokens (8, 16, 32, 64 at a time; groups of 16 to 256 weight rows, one or several per CTA; K with and without whole
+# blocks of 128), split K, single and paired tiles, ragged edges in every dimension
+SHAPES = [(1, 1, 16), (1, 256, 128), (1, 6144, 4096), (1, 2112, 7168), (1, 28672, 1024), (2, 33, 48), (3, 100003, 272), (7, 130, 2064),
+          (8, 40000, 528), (9, 37889, 256), (16, 28672, 4096), (17, 75777, 384), (20, 24576, 1040), (24, 15000, 784), (31, 4096, 4096),
+          (32, 300, 16), (32, 28672, 2048), (33, 208, 496), (50, 4096, 4096), (64, 9472, 208), (64, 9473, 208), (64, 24576, 1040),
+          (83, 7744, 3888), (100, 2112, 7168), (128, 4096, 14336), (129, 144, 144), (130, 4097, 528), (257, 9500, 256),
+          (1024, 6144, 4096), (1037, 6145, 4096), (4099, 8191, 512), (8192, 8192, 1024)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
 def test_per_token_per_channel(m, n, k):
     a, b, a_s, b_s, _ = _operands(m, n, k)
     _check(flag_gems.w8a8_int8_matmul(a, b, a_s, b_s), _definition(a, b, a_s, b_s))
+
+
+@pytest.mark.parametrize("m", [65, 129, 300, 513, 777, 1037, 1300, 3000])
+@pytest.mark.parametrize("n", [515, 2112, 4100, 6144, 7168, 11008])
+def test_tiles_of_every_width(m, n):
+    """Row counts and widths between which the tile's width and kind change; 8 blocks of K and a short one."""
+    a, b, a_s, b_s, g = _operands(m, n, 1040, seed=n)
+    c = torch.randn(n, device="cuda", generator=g).half()
+    _check(flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, c, torch.float16), _definition(a, b, a_s, b_s), c)
+
+
+@pytest.mark.parametrize("m", [1, 20, 200])
+@pytest.mark.parametrize("n", [4096, 30000])
+def test_operands_that_the_kernel_before_writes(m, n):
+    """The product may be launched while its operands are still being written, into memory that held others before."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    w, x = torch.randn(n, 2048, device="cuda", generator=g).bfloat16(), torch.randn(m, 2048, device="cuda", generator=g).bfloat16()
+    kept = []
+    for i in range(8):
+        a, a_s = flag_gems.per_token_quant_int8(x)
+        b, b_s = flag_gems.per_token_quant_int8(w)
+        c = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s)
+        kept.append((a.clone(), b.clone(), a_s.clone(), b_s.clone(), c))
+        del a, b, a_s, b_s
+        x, w = x.roll(1, 1), w.roll(3, 0) * 1.25
+    for a, b, a_s, b_s, c in kept:
+        _check(c, _definition(a, b, a_s, b_s))
+
+
+@pytest.mark.parametrize("m", [1, 5, 12, 31, 60])
+def test_few_tokens_twice_at_once(m):
+    """The same call on two streams, and one after another without a wait between."""
+    ops = [_operands(m, 20000 + 16 * i, 2048, seed=i) for i in range(4)]
+    want = [_definition(*o[:4]) for o in ops]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for r in range(3):
+        for i, o in enumerate(ops):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append((i, flag_gems.w8a8_int8_matmul(*o[:4])))
+    torch.cuda.synchronize()
+    for i, c in got:
+        _check(c, want[i])
+    assert _cabi.device_status() == 0
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
