@@ -89,7 +89,7 @@ struct FgSkinny {
     int64_t M, N, K, ld_a, ld_b, ld_c;
     int sa_mode, sb_mode, out_dtype, bias_dtype, bias_after_round;
 };
-bool fg_int8_is_skinny(int64_t M, int64_t N);
+bool fg_int8_is_skinny(int64_t M);
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st);
 
 // The rows of a grouped product's result that follow its last group, to be filled with zeros (c NULL: left as they are).

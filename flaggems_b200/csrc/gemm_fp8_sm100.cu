@@ -295,7 +295,7 @@ __device__ __forceinline__ TileCoord tile_coord(int t, int num_m, int num_n) {
 // fewer tiles than SMs and the job is to pull the weights from HBM with every SM.
 // OPK (operand kind): 0 = e4m3 (kind::f8f6f4); 1 = signed 8-bit integers with 32-bit integer accumulators
 // (kind::i8) for the int8 w8a8 products, dense and grouped (the epilogue converts the accumulators to fp32 and
-// applies the per-row x per-column scales; split-K adds the integers, so any split gives the same bits); 2 / 3 = bf16 / f16 (kind::f16) for the unquantised and
+// applies the per-row x per-column scales); 2 / 3 = bf16 / f16 (kind::f16) for the unquantised and
 // weight-only-quantised expert GEMMs.  The main loop is written in bytes (a K block is 128 bytes of a
 // K-major row, an MMA consumes 32 of them), so a 16-bit product of K elements runs as 2K bytes.
 template <int BN, bool BLOCK_SCALED, bool FUSE_SILU, bool SMALL_A, bool SPLITK, bool PAIR = false, bool ASTORE = false,
@@ -306,9 +306,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     using C = Cfg<BN, SMALL_A, PAIR, ASTORE, !BLOCK_SCALED && !SPLITK>;
     static_assert(!ASTORE || (BLOCK_SCALED && !SPLITK), "the store warp serves the block-scaled tiles");
     constexpr bool INT8 = OPK == 1;
-    static_assert(OPK == 0 || !BLOCK_SCALED, "block scales are for e4m3 operands");
-    static_assert(OPK == 0 || !SMALL_A, "int8 products of so few rows are int8_skinny.cu's");
-    static_assert(OPK < 2 || !SPLITK, "16-bit operands serve the grouped tiles");
+    // int8 products of up to 128 rows are int8_skinny.cu's; 16-bit operands serve the grouped tiles
+    static_assert(OPK == 0 || (!BLOCK_SCALED && !SPLITK && !SMALL_A), "these are built for e4m3 operands");
     // accumulator word -> fp32
     auto acc_f = [](uint32_t raw) -> float {
         if constexpr (INT8) return __int2float_rn((int)raw);
@@ -319,7 +318,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     static_assert(!FUSE_SILU || BN >= 128, "fused SiLU needs a tile of at least 128 columns");
     constexpr int STAGES = C::STAGES;
     // Output columns per tile.  int8 tiles may be narrower than BN, so that their number fits the SMs.
-    constexpr bool ANY_WIDTH = INT8 && !FUSE_SILU && !SPLITK && BN >= 128;
+    constexpr bool ANY_WIDTH = INT8 && !FUSE_SILU && BN >= 128;
     constexpr int FULL_TILE_N = FUSE_SILU ? BN / 2 : BN;
     const int OUT_TILE_N = ANY_WIDTH ? p.tile_n : FULL_TILE_N;
     // DUAL (block-scaled wide tiles): warps 1 and 2 issue the MMAs of alternate K blocks.  A K block's
@@ -1147,13 +1146,12 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             const int n_epi = C::EPI_WARPS * 32;
             for (int idx = threadIdx.x - C::FIRST_EPI_WARP * 32; idx < rows * vec_per_row; idx += n_epi) {
                 const int r = idx / vec_per_row, c = c_first + (idx % vec_per_row) * 4;
-                using Part = std::conditional_t<INT8, int4, float4>;
-                Part sum{};
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int q = 0; q < k_slices; ++q) {
-                    const Part v = *reinterpret_cast<const Part*>(part[q] + (size_t)r * (BN + 4) + c);
+                    const float4 v = *reinterpret_cast<const float4*>(part[q] + (size_t)r * (BN + 4) + c);
                     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
                 }
-                float o[4] = {(float)sum.x, (float)sum.y, (float)sum.z, (float)sum.w};
+                float o[4] = {sum.x, sum.y, sum.z, sum.w};
                 const int64_t row = (int64_t)m0 + r;
                 if constexpr (!BLOCK_SCALED) {
                     const float sa = p.sa_mode == FG_SCALE_VECTOR ? p.sa[row] : p.sa[0];
@@ -1236,7 +1234,7 @@ int fg_byte_map(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint
 namespace {
 
 // How many clusters of `slices` CTAs of the split-K kernel fit on the device at once (cached).
-template <int BN, bool BS, int OPK = 0>
+template <int BN, bool BS>
 int max_resident_clusters(int slices) {
     static int table[64][9];
     static std::mutex mu;
@@ -1244,7 +1242,7 @@ int max_resident_clusters(int slices) {
     int* cache = table[fg_device_index()];
     if (cache[slices]) return cache[slices];
     using C = Cfg<BN, false>;
-    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true, false, false, OPK>;
+    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true>;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(slices * 64), 1, 1);
@@ -1266,11 +1264,11 @@ int max_resident_clusters(int slices) {
     return n;
 }
 
-template <int BN, bool BS, int OPK = 0>
+template <int BN, bool BS>
 int launch_splitk(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, int tiles, int slices,
                   cudaStream_t st) {
     using C = Cfg<BN, false>;
-    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true, false, false, OPK>;
+    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true>;
     static bool attr_done[64];
     static std::mutex mu;
     {
@@ -1360,13 +1358,14 @@ int launch_inst(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& 
     return FG_OK;
 }
 
-// Tile of a dense int8 product: the width and the kind (one CTA per 128 rows, or a CTA pair per 256) with the least estimated time,
-// which is the number of waves of tiles times what a block of K takes, which hardly depends on the width below 256
-// (the ring's round trip; above, the 64 bytes per cycle that an SM takes in).  So a narrower tile pays where it saves a
-// wave, and a pair where a tile's K is long enough for its dearer start.  The constants (ns) are fitted to 5 weights x 12 row counts
-// x 11 tiles on this chip, and the choices are within 5 % of the best of the 11.  Measured, 256-wide single / 256-wide pair / this:
-// 1037 x 6144 x 4096 32.3 / 28.7 / 27.0 us (pairs of 224 columns, two full waves), 300 x 7168 x 2048 13.3 / 13.2 / 12.0 (single,
-// 160), 777 x 4096 x 14336 51.1 / 44.1 / 44.1, 1037 x 4096 x 14336 52.3 / 75.0 / 52.3, 128 x 6144 x 4096 18.9 / 17.2 / 15.1 (single, 96).
+// Tile of a dense int8 product of more than 128 rows: the width and the kind (one CTA per 128 rows, or a CTA pair per
+// 256) with the least estimated time.  That is the number of waves of tiles times what a block of K takes, which hardly
+// depends on the width below 256 (the ring's round trip; above, the 64 bytes per cycle that an SM takes in).  So a narrower
+// tile pays where it saves a wave, and a pair where a tile's K is long enough for its dearer start.  The constants (ns) are
+// fitted to 5 weights x 12 row counts x 11 tiles; the choices are within 6 % of the best of the 11.  Measured, 256-wide
+// single / 256-wide pair / this: 1037 x 6144 x 4096 32.3 / 28.7 / 27.0 us (pairs of 224 columns, two full waves),
+// 300 x 7168 x 2048 13.3 / 13.2 / 12.0 (single, 160), 777 x 4096 x 14336 51.1 / 44.1 / 44.1, 1037 x 4096 x 14336 52.3 /
+// 75.0 / 52.3, 256 x 6144 x 4096 19.6 / 17.5 / 15.4 (single, 96).
 struct Int8Tile {
     bool pair;
     int width;
@@ -1384,14 +1383,10 @@ Int8Tile int8_tile(int64_t M, int64_t N, int64_t k_blocks, int sms) {
     };
     for (int width = 256; width >= 96; width -= 32) offer(false, width, 4000, 290 + 130 * width / 256);
     offer(false, 64, 4000, 285);
-    if (M > BLOCK_M)
+    if (pair_enabled())
         for (int width = 256; width >= 128; width -= 32) offer(true, width, 5500, 265 + 80 * width / 256);
     return best;
 }
-// Up to 128 rows and up to here in K the tiles above beat split K, whose reduction through the cluster costs about as much
-// as 40 blocks: 128 x 6144 x 4096 15.1 / 20.8 us, 128 x 7168 x 2048 10.0 / 18.7, but 128 x 2112 x 7168 21.0 / 17.6 and
-// 128 x 4096 x 14336 36.6 / 30.0.
-constexpr int SPLITK_MIN_K_INT8 = 5120;
 
 // Rows of both operands in bytes.
 int check_operands(const void* a, const void* b, int64_t K, int64_t ld_a, int64_t ld_b) {
@@ -1443,9 +1438,7 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
         const int64_t nkb = fg_cdiv(p.K, BLOCK_K);
         for (int cand = 8; cand >= 2; cand /= 2) {
             const int64_t per = fg_cdiv(nkb, cand);
-            const int resident = p.int8 == 1
-                ? (wide == 256 ? max_resident_clusters<256, false, 1>(cand) : max_resident_clusters<128, false, 1>(cand))
-                : wide == 256
+            const int resident = wide == 256
                 ? (block_scaled ? max_resident_clusters<256, true>(cand) : max_resident_clusters<256, false>(cand))
                 : (block_scaled ? max_resident_clusters<128, true>(cand) : max_resident_clusters<128, false>(cand));
             if (wide_tiles <= resident && per >= 2 && (cand - 1) * per < nkb) {
@@ -1464,13 +1457,10 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     p.tile_n = fuse_silu ? bn / 2 : bn;
     bool int8_pair = false;
     if (p.int8 == 1 && !p.grouped) {
-        if (k_slices > 1 && p.K <= SPLITK_MIN_K_INT8) k_slices = 1;
-        if (k_slices == 1) {
-            const Int8Tile t = int8_tile(p.M, p.n_out, fg_cdiv(p.K, BLOCK_K), sms);
-            int8_pair = t.pair;
-            p.tile_n = t.width;
-            bn = t.width > 128 || t.pair ? 256 : t.width > 64 ? 128 : 64;
-        }
+        const Int8Tile t = int8_tile(p.M, p.n_out, fg_cdiv(p.K, BLOCK_K), sms);
+        int8_pair = t.pair;
+        p.tile_n = t.width;
+        bn = t.width > 128 || t.pair ? 256 : t.width > 64 ? 128 : 64;
     }
     const int64_t pair_tiles = fg_cdiv(p.M, 2 * BLOCK_M) * fg_cdiv(p.n_out, fuse_silu ? 128 : int8_pair ? p.tile_n : 256);
     const bool pair = int8_pair || grouped_pair || (p.int8 == 0 && !p.grouped && !fuse_silu && !block_scaled && bn == 256 && k_slices == 1 &&
@@ -1504,11 +1494,7 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     if (p.int8) {
         FG_REQUIRE(!block_scaled && (p.int8 == 1 || p.grouped), FG_ERR_UNSUPPORTED,
                    "int8 operands take no block scales, and 16-bit operands are built for the grouped expert GEMMs");
-        if (!p.grouped) {
-            if (k_slices > 1) return bn == 256 ? launch_splitk<256, false, 1>(ta, tb, p, t, k_slices, st)
-                                               : launch_splitk<128, false, 1>(ta, tb, p, t, k_slices, st);
-            if (bn == 64) return launch_inst<64, false, false, false, false, 1>(ta, tb, p, t, st);
-        }
+        if (bn == 64) return launch_inst<64, false, false, false, false, 1>(ta, tb, p, t, st);
         auto by_kind = [&](auto bn_tag, auto silu_tag) -> int {
             constexpr int B = decltype(bn_tag)::value;
             constexpr bool S = decltype(silu_tag)::value;
@@ -1591,7 +1577,7 @@ int scaled_mm_common(int operand, void* c, const void* a, const void* b, const f
     p.bias_dtype = bias_dtype;
     p.block_rows = BLOCK_M;
     p.int8 = operand;
-    if (operand == 1 && fg_int8_is_skinny(M, N)) {
+    if (operand == 1 && fg_int8_is_skinny(M)) {
         const int rc = check_operands(a, b, K, ld_a, ld_b);
         if (rc != FG_OK) return rc;
         return fg_int8_skinny(FgSkinny{c, (const int8_t*)a, (const int8_t*)b, sa, sb, bias, M, N, K, ld_a, ld_b, ld_c, sa_mode, sb_mode,
@@ -1640,7 +1626,6 @@ int fg_scaled_mm_int8(void* c, const void* a, const void* b, const float* sa, co
     return scaled_mm_common(1, c, a, b, sa, sb, bias, bias_dtype, M, N, K, ld_a, ld_b, ld_c, sa_mode, sb_mode, out_dtype,
                             bias_after_round, stream);
 }
-
 
 int fg_block_scaled_mm_fp8(void* c, const void* a, const void* b, const float* a_s, const float* b_s, int64_t M,
                            int64_t N, int64_t K, int64_t ld_a, int64_t ld_b, int64_t ld_c, int64_t ld_as,

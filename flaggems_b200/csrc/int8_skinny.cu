@@ -1,18 +1,26 @@
-// Products of few int8 tokens and a large int8 weight: C[m, n] = sum_k A[m, k] B[n, k], scaled per token and channel.
+// Products of few int8 tokens (up to 128) and a large int8 weight: C[m, n] = sum_k A[m, k] B[n, k], scaled per token and channel.
 //
-// With so few tokens the weight's bytes are all the work, and the job is to keep enough of them under way on every
+// With so few tokens the weight's bytes are most of the work, and the job is to keep enough of them under way on every
 // SM, from the first cycle to the last.  A CTA owns groups of weight rows, as many per group as it takes for the groups to
 // cover the SMs once (or a whole number of times); one thread streams them by TMA into a ring that fills the shared
-// memory, across the ends of groups, so that no epilogue interrupts the stream.  Eight warps multiply with mma.m16n8k32
-// (weight rows as M, tokens as N): they share a stage's KB blocks of K and its strips of 16 rows, and the sums, whole
-// numbers, are added in shared memory in any order.  The tensor cores of tcgen05 would be idle here whatever they are
-// fed with, and need the tokens padded to 128 rows and the weight cut in tiles of 256 rows, which leaves SMs without one.
+// memory, across the ends of groups, so that no epilogue interrupts the stream.  Between weights of 117 and 176 MB
+// that runs at 6.5 TB/s, the rate of a copy; 4 us are spent around it.  What multiplies depends on the tokens:
 //
-// K is a sum, so its order is free: lane (g, t) of a warp takes bytes [32 t, 32 t + 32) of a block's rows, for the weight
-// and the tokens alike, as two 16-byte loads without bank conflicts, not the 4-byte pieces that the instruction's layout names.
+//   up to 16 (or 32)  eight warps with mma.m16n8k32, weight rows as M and tokens as N; they share a stage's KB blocks of K and
+//                     its strips of 16 rows, and the sums, whole numbers, are added in shared memory in any order;
+//   up to 128         one thread with tcgen05 (kind::i8), tokens as M and weight rows as N, into TMEM.
+//
+// Against the tiles that serve more tokens (128 x 256 and the like, with K split over a cluster) this saves the padding to 128
+// rows, the SMs that 256-row tiles leave without one, and the reduction: 1 x 6144 x 4096 6.3 us (11.0), 16 x 28672 x 4096 22.7
+// (26.6), 64 x 6144 x 4096 10.0 (15.9), 128 x 2112 x 7168 13.1 (17.6), 128 x 7168 x 2048 7.1 (18.7).
+//
+// K is a sum, so its order is free: with mma.m16n8k32, lane (g, t) of a warp takes bytes [32 t, 32 t + 32) of a block's rows,
+// for the weight and the tokens alike, as two 16-byte loads without bank conflicts, not the 4-byte pieces that the
+// instruction's layout names.
 #include <cuda.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "ptx_sm100.cuh"
@@ -25,14 +33,17 @@ constexpr int WARPS = 8;  // that multiply; one more fetches
 constexpr int THREADS = 32 * (WARPS + 1);
 constexpr int BLOCK_K = 128;
 constexpr int MAX_ROWS = 256;
+constexpr int MAX_TOKENS = 128;
 constexpr int MAX_STAGES = 16;
-constexpr int SMEM_BYTES = 224 * 1024;  // ring, sums and alignment
+constexpr int SMEM_BYTES = 224 * 1024;         // ring, sums and alignment
+constexpr int STREAM_SMEM_BYTES = 220 * 1024;  // ring, rows behind it and alignment; 5 KB are static
 
 struct StreamArgs {
     FgSkinny p;
     int rows;    // per group, a multiple of 16
     int groups;
     int stages;
+    int token_rows;  // int8_stream_kernel: rows of the tokens' box, a multiple of 8
     int wide;  // one load brings all KB blocks of a stage (K a multiple of 128); otherwise each has its own
     unsigned int* status;
 };
@@ -55,12 +66,59 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A barrier of the multiplying warps that also tells all of them whether any of them failed.
+// A barrier of THREADS threads that also tells all of them whether any of them failed.
+template <int THREADS>
 __device__ __forceinline__ bool any_failed(bool failed) {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"((uint32_t)failed), "n"(32 * WARPS) : "memory");
+                 : "=r"(r) : "r"((uint32_t)failed), "n"(THREADS) : "memory");
     return r != 0u;
+}
+
+// A wait ran out somewhere: what is still under way lands before the CTA ends.
+__device__ void drain(uint64_t* full_bar, int stages, int issued) {
+    uint32_t alone = 0u;
+    for (int j = issued > stages ? issued - stages : 0; j < issued; ++j)
+        mbar_wait(&full_bar[j % stages], (uint32_t)(j / stages) & 1u, &alone, nullptr, 0, 100000000ull);
+}
+
+// `cols` (up to 32) consecutive values of row m from column n on.
+__device__ __forceinline__ void store_row(const FgSkinny& p, int64_t m, int64_t n, const float (&v)[32], int cols) {
+    const int64_t at = m * p.ld_c + n;
+    if (p.out_dtype == FG_DTYPE_F32) {
+        float* o = reinterpret_cast<float*>(p.c) + at;
+        const bool vec = (reinterpret_cast<uintptr_t>(o) & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            if (vec && i + 4 <= cols) {
+                *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j < cols) o[i + j] = v[i + j];
+            }
+        }
+        return;
+    }
+    uint16_t* o = reinterpret_cast<uint16_t*>(p.c) + at;
+    const bool vec = (reinterpret_cast<uintptr_t>(o) & 15) == 0, bf16 = p.out_dtype == FG_DTYPE_BF16;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+            const __half2 h = __floats2half2_rn(v[i + 2 * j], v[i + 2 * j + 1]);
+            w[j] = bf16 ? *reinterpret_cast<const uint32_t*>(&b) : *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (vec && i + 8 <= cols) {
+            *reinterpret_cast<uint4*>(o + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < cols) o[i + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+        }
+    }
 }
 
 // NT: tiles of eight tokens.  KB: blocks of K per stage; 8 / KB warps share the strips of 16 rows of a block, up to SPW
@@ -126,11 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
                         phase ^= 1u;
                     }
                 }
-            if (*abort_flag) {  // a wait ran out somewhere: what is still under way lands before the CTA ends
-                uint32_t alone = 0u;
-                for (int j = issued > a.stages ? issued - a.stages : 0; j < issued; ++j)
-                    mbar_wait(&full_bar[j % a.stages], (uint32_t)(j / a.stages) & 1u, &alone, nullptr, 0, 100000000ull);
-            }
+            if (*abort_flag) drain(full_bar, a.stages, issued);
         }
         __syncwarp();
         fg_pdl_trigger();  // every load has been issued
@@ -202,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
                         if (m < p.M) atomicAdd(&sums[m * a.rows + 16 * strip + 8 * (i >> 1) + g], acc[s][j][i]);
                     }
             }
-            if (any_failed(!ok)) break;
+            if (any_failed<32 * WARPS>(!ok)) break;
             if (mine) {
                 for (int m = 0; m < p.M; ++m) {
                     float v = sb * (sa_s[m] * (float)sums[m * a.rows + r]);
@@ -214,10 +268,217 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
                     else reinterpret_cast<float*>(p.c)[at] = v;
                 }
             }
-            if (grp + gridDim.x < a.groups) any_failed(false);  // the sums are zeros again
+            if (grp + gridDim.x < a.groups) any_failed<32 * WARPS>(false);  // the sums are zeros again
         }
     }
     __syncthreads();
+}
+
+// The same stream for more tokens, multiplied by tcgen05 (kind::i8): tokens are the 128 rows of the accumulator in TMEM, the
+// group's weight rows its columns.  Only the token rows that exist are fetched; the instruction reads 128, and what the
+// others hold reaches accumulator rows that nobody reads.  Warp 0 fetches, warp 1 multiplies, warps 4 to 7 finish a
+// group (two accumulators: the next group is multiplied meanwhile).
+template <int KB>
+__global__ void __launch_bounds__(256, 1) int8_stream_kernel(const __grid_constant__ CUtensorMap tm_w,
+                                                             const __grid_constant__ CUtensorMap tm_x, const StreamArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint32_t abort_word, tmem_slot;
+    __shared__ __align__(16) float col_scale[2][MAX_ROWS];
+    __shared__ float col_bias[2][MAX_ROWS];
+    const FgSkinny& p = a.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int x_block = a.token_rows * BLOCK_K, w_block = a.rows * BLOCK_K, stage_bytes = KB * (x_block + w_block);
+    const int steps = ((int)p.K + KB * BLOCK_K - 1) / (KB * BLOCK_K);
+    const int quads = ((int)p.M + 31) / 32;                         // warps of the epilogue that hold tokens
+    const int acc_cols = (a.rows + 31) / 32 * 32;                   // of one accumulator
+    const uint32_t tmem_cols = 2 * acc_cols <= 64 ? 64 : 2 * acc_cols <= 128 ? 128 : 2 * acc_cols <= 256 ? 256 : 512;
+    volatile uint32_t* abort_flag = &abort_word;
+    if (warp == 0 && lane == 0) {
+        if (a.wide)  // as above: as far as L2 while the kernel before this one drains
+            for (int step = 0; step < min(a.stages, steps); ++step) tma_prefetch_3d(&tm_w, 0, blockIdx.x * a.rows, step * KB);
+        for (int s = 0; s < a.stages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], quads);
+        }
+        abort_word = 0u;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_slot, tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    fg_pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int grp = blockIdx.x; grp < a.groups && ok; grp += gridDim.x)
+                for (int step = 0; step < steps; ++step) {
+                    ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, a.status, 22);
+                    if (!ok) break;
+                    uint8_t* to = ring + (size_t)stage * stage_bytes;
+                    mbar_arrive_expect_tx(&full_bar[stage], (uint32_t)stage_bytes);
+                    if (a.wide) {
+                        tma_load_3d(to, &tm_x, &full_bar[stage], 0, 0, step * KB);
+                        tma_load_3d(to + KB * x_block, &tm_w, &full_bar[stage], 0, grp * a.rows, step * KB);
+                    } else {
+#pragma unroll 1
+                        for (int b = 0; b < KB; ++b) {
+                            tma_load_3d(to + b * x_block, &tm_x, &full_bar[stage], (step * KB + b) * BLOCK_K, 0, 0);
+                            tma_load_3d(to + KB * x_block + b * w_block, &tm_w, &full_bar[stage], (step * KB + b) * BLOCK_K, grp * a.rows, 0);
+                        }
+                    }
+                    ++issued;
+                    if (++stage == a.stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            if (*abort_flag) drain(full_bar, a.stages, issued);
+        }
+        __syncwarp();
+        fg_pdl_trigger();  // every load has been issued
+    } else if (warp == 1) {
+        const uint32_t idesc = umma_idesc_s8_s32(128, a.rows);
+        int stage = 0;
+        uint32_t phase = 0, round = 0;
+        bool ok = true;
+        for (int grp = blockIdx.x; grp < a.groups && ok; grp += gridDim.x, ++round) {
+            const uint32_t buf = round & 1u, d = tmem + buf * acc_cols;
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((round >> 1) & 1u) ^ 1u, abort_flag, a.status, 23));
+            if (!ok) break;
+            tc_fence_after_sync();
+            for (int step = 0; step < steps; ++step) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, a.status, 24));
+                if (!ok) break;
+                if (elect_one()) {
+                    const uint32_t x_addr = smem_u32(ring + (size_t)stage * stage_bytes), w_addr = x_addr + KB * x_block;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) {
+                        const uint64_t x_desc = umma_desc_k_sw128(x_addr + b * x_block), w_desc = umma_desc_k_sw128(w_addr + b * w_block);
+#pragma unroll
+                        for (int k = 0; k < BLOCK_K / 32; ++k)
+                            umma_i8(d, x_desc + (uint64_t)(2 * k), w_desc + (uint64_t)(2 * k), idesc, step > 0 || b > 0 || k > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&empty_bar[stage]);
+                    if (step == steps - 1) umma_commit(&acc_full[buf]);
+                }
+                __syncwarp();
+                if (++stage == a.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        const int quad = warp & 3, tid = (int)threadIdx.x - 128, m = quad * 32 + lane;
+        const bool tokens = quad < quads, mine = m < p.M;
+        const float sa = p.sa[p.sa_mode == FG_SCALE_VECTOR && mine ? m : 0];
+        uint32_t round = 0;
+        bool ok = true;
+        for (int grp = blockIdx.x; grp < a.groups; grp += gridDim.x, ++round) {
+            const uint32_t buf = round & 1u;
+            const int64_t n0 = (int64_t)grp * a.rows;
+            for (int r = tid; r < a.rows; r += 128) {
+                const int64_t n = n0 + r < p.N ? n0 + r : p.N - 1;
+                col_scale[buf][r] = p.sb[p.sb_mode == FG_SCALE_VECTOR ? n : 0];
+                col_bias[buf][r] = p.bias ? load_bias(p.bias, p.bias_dtype, n) : 0.0f;
+            }
+            if (any_failed<128>(!ok)) break;
+            if (!tokens) continue;
+            ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (round >> 1) & 1u, abort_flag, a.status, 25));
+            if (!ok) continue;
+            tc_fence_after_sync();
+            const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + buf * acc_cols;
+            for (int c = 0; c < a.rows; c += 32) {
+                uint32_t raw[32];
+                tmem_ld_32x32b_x32(acc + c, raw);
+                tmem_ld_wait();
+                const int cols = (int)min((int64_t)min(32, a.rows - c), p.N - n0 - c);
+                if (!mine || cols <= 0) continue;
+                float v[32];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 s = *reinterpret_cast<const float4*>(&col_scale[buf][c + 4 * q]);
+                    v[4 * q] = s.x * (sa * (float)(int)raw[4 * q]);
+                    v[4 * q + 1] = s.y * (sa * (float)(int)raw[4 * q + 1]);
+                    v[4 * q + 2] = s.z * (sa * (float)(int)raw[4 * q + 2]);
+                    v[4 * q + 3] = s.w * (sa * (float)(int)raw[4 * q + 3]);
+                }
+                if (p.bias) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = (p.bias_after_round ? rounded(v[i], p.out_dtype) : v[i]) + col_bias[buf][c + i];
+                }
+                store_row(p, m, n0 + c, v, cols);
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, tmem_cols);
+    }
+}
+
+int byte_maps(StreamArgs& a, int kb, int token_rows, CUtensorMap* tm_w, CUtensorMap* tm_x) {
+    const FgSkinny& p = a.p;
+    a.wide = p.K % BLOCK_K == 0;
+    int rc;
+    if (a.wide) {  // blocks of 128 bytes as the last dimension
+        const uint64_t blocks = (uint64_t)(p.K / BLOCK_K);
+        rc = fg_byte_map(tm_w, p.b, BLOCK_K, (uint64_t)p.N, blocks, (uint64_t)p.ld_b, BLOCK_K, (uint32_t)a.rows, 3, (uint32_t)kb);
+        if (rc == FG_OK) rc = fg_byte_map(tm_x, p.a, BLOCK_K, (uint64_t)p.M, blocks, (uint64_t)p.ld_a, BLOCK_K, (uint32_t)token_rows, 3, (uint32_t)kb);
+    } else {
+        rc = fg_byte_map(tm_w, p.b, (uint64_t)p.K, (uint64_t)p.N, 1, (uint64_t)p.ld_b, (uint64_t)p.ld_b * p.N, (uint32_t)a.rows, 3);
+        if (rc == FG_OK) rc = fg_byte_map(tm_x, p.a, (uint64_t)p.K, (uint64_t)p.M, 1, (uint64_t)p.ld_a, (uint64_t)p.ld_a * p.M, (uint32_t)token_rows, 3);
+    }
+    return rc;
+}
+
+template <int KB>
+int launch_stream(StreamArgs& a, cudaStream_t st) {
+    const FgSkinny& p = a.p;
+    auto kernel = int8_stream_kernel<KB>;
+    static bool attr_done[64];
+    static std::mutex mu;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        bool& done = attr_done[fg_device_index()];
+        if (!done) {
+            FG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STREAM_SMEM_BYTES));
+            done = true;
+        }
+    }
+    const int grid = a.groups < fg_num_sms() ? a.groups : fg_num_sms();
+    const int64_t stage = (int64_t)KB * (a.rows + a.token_rows) * BLOCK_K;
+    const int64_t all = fg_cdiv(p.K, KB * BLOCK_K) * fg_cdiv(a.groups, grid);
+    const int64_t pad = 128 * BLOCK_K;  // the instruction reads 128 rows of tokens from the last stage too
+    int64_t stages = (STREAM_SMEM_BYTES - 1024 - pad) / stage;
+    if (stages > MAX_STAGES) stages = MAX_STAGES;
+    if (stages > all) stages = all;
+    FG_REQUIRE(stages >= 1, FG_ERR_UNSUPPORTED, "a stage of %lld bytes does not fit", (long long)stage);
+    a.stages = (int)stages;
+    CUtensorMap tm_w, tm_x;
+    const int rc = byte_maps(a, KB, a.token_rows, &tm_w, &tm_x);
+    if (rc != FG_OK) return rc;
+    FG_CUDA(fg_launch(kernel, (unsigned)grid, 256, (size_t)(stages * stage + pad + 1024), st, 1, tm_w, tm_x, a));
+    return FG_OK;
 }
 
 template <int NT, int SPW, int KB>
@@ -243,17 +504,8 @@ int launch(StreamArgs& a, cudaStream_t st) {
     if (stages > all) stages = all;
     FG_REQUIRE(stages >= 1, FG_ERR_UNSUPPORTED, "a stage of %lld bytes does not fit", (long long)stage);
     a.stages = (int)stages;
-    a.wide = p.K % BLOCK_K == 0;
     CUtensorMap tm_w, tm_x;
-    int rc;
-    if (a.wide) {  // blocks of 128 bytes as the last dimension
-        const uint64_t blocks = (uint64_t)(p.K / BLOCK_K);
-        rc = fg_byte_map(&tm_w, p.b, BLOCK_K, (uint64_t)p.N, blocks, (uint64_t)p.ld_b, BLOCK_K, (uint32_t)a.rows, 3, KB);
-        if (rc == FG_OK) rc = fg_byte_map(&tm_x, p.a, BLOCK_K, (uint64_t)p.M, blocks, (uint64_t)p.ld_a, BLOCK_K, 8 * NT, 3, KB);
-    } else {
-        rc = fg_byte_map(&tm_w, p.b, (uint64_t)p.K, (uint64_t)p.N, 1, (uint64_t)p.ld_b, (uint64_t)p.ld_b * p.N, (uint32_t)a.rows, 3);
-        if (rc == FG_OK) rc = fg_byte_map(&tm_x, p.a, (uint64_t)p.K, (uint64_t)p.M, 1, (uint64_t)p.ld_a, (uint64_t)p.ld_a * p.M, 8 * NT, 3);
-    }
+    const int rc = byte_maps(a, KB, 8 * NT, &tm_w, &tm_x);
     if (rc != FG_OK) return rc;
     const size_t smem = (size_t)(stages * stage + sums);
     FG_CUDA(fg_launch(kernel, (unsigned)grid, THREADS, smem, st, 1, tm_w, tm_x, a));
@@ -261,21 +513,31 @@ int launch(StreamArgs& a, cudaStream_t st) {
 }
 
 // Stages of 20 to 48 KB: the lower a group, the more blocks of K.
-template <int NT>
-int launch_rows(StreamArgs& a, cudaStream_t st) {
-    if (a.rows <= 16) return launch<NT, 1, 8>(a, st);
-    if (a.rows <= 32) return launch<NT, 2, 8>(a, st);
-    if (a.rows <= 64) return launch<NT, 2, 4>(a, st);
-    if constexpr (NT < 8) {
-        if (a.rows <= 128) return launch<NT, 2, 2>(a, st);
-        return launch<NT, 2, 1>(a, st);
-    }
-    fg_set_error("groups of %d rows are built for up to 32 tokens", a.rows);
-    return FG_ERR_UNSUPPORTED;
+int launch_registers(StreamArgs& a, cudaStream_t st) {
+    auto by_rows = [&](auto nt) -> int {
+        constexpr int NT = decltype(nt)::value;
+        if (a.rows <= 16) return launch<NT, 1, 8>(a, st);
+        if (a.rows <= 32) return launch<NT, 2, 8>(a, st);
+        if constexpr (NT <= 2) {
+            if (a.rows <= 64) return launch<NT, 2, 4>(a, st);
+            if (a.rows <= 128) return launch<NT, 2, 2>(a, st);
+            return launch<NT, 2, 1>(a, st);
+        }
+        fg_set_error("groups of %d rows are built for up to 16 tokens", a.rows);
+        return FG_ERR_UNSUPPORTED;
+    };
+    const int64_t m = a.p.M;
+    return m <= 8 ? by_rows(std::integral_constant<int, 1>()) : m <= 16 ? by_rows(std::integral_constant<int, 2>())
+                                                                        : by_rows(std::integral_constant<int, 4>());
 }
 
-// Rows per group, as many groups as that gives: as few rounds of groups as their height allows, and in those all
-// groups of one height.
+int launch_tensor_memory(StreamArgs& a, cudaStream_t st) {
+    a.token_rows = (int)((a.p.M + 7) / 8 * 8);
+    const int rows = a.rows + a.token_rows;
+    return rows <= 96 ? launch_stream<4>(a, st) : rows <= 192 ? launch_stream<2>(a, st) : launch_stream<1>(a, st);
+}
+
+// Rows per group: as few rounds of groups as their height allows, and in those all groups of one height.
 int group_rows(int64_t N) {
     const int64_t rounds = fg_cdiv(N, (int64_t)MAX_ROWS * fg_num_sms());
     return (int)(fg_cdiv(fg_cdiv(N, rounds * fg_num_sms()), 16) * 16);
@@ -283,19 +545,19 @@ int group_rows(int64_t N) {
 
 }  // namespace
 
-// Up to 32 tokens the weight streams at the rate of HBM (6.5 TB/s between a 117 MB and a 176 MB weight, and 4 us around
-// that); above, mma.sync runs out (0.4 PFLOP/s): with groups of up to 64 rows, where the tiles of tcgen05 are
-// slower still, up to 64 tokens.  Measured, this against the tcgen05 tiles: M = 1, N x K = 6144 x 4096 6.3 / 11.0 us, 28672 x 4096
-// 21.4 / 25.5, 24576 x 7168 31.0 / 36.8; M = 32 9.4 / 13.4, 25.2 / 26.5, 37.6 / 37.9; M = 64 14.7 / 15.9, 38.8 / 27.1,
-// 56.0 / 38.8.
-bool fg_int8_is_skinny(int64_t M, int64_t N) { return M <= 32 || (M <= 64 && group_rows(N) <= 64); }
+bool fg_int8_is_skinny(int64_t M) { return M <= MAX_TOKENS; }
 
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st) {
-    FG_REQUIRE(p.M > 0 && p.N > 0 && fg_int8_is_skinny(p.M, p.N) && p.K > 0 && p.K % 16 == 0, FG_ERR_UNSUPPORTED, "bad sizes");
+    FG_REQUIRE(p.M > 0 && p.N > 0 && p.M <= MAX_TOKENS && p.K > 0 && p.K % 16 == 0, FG_ERR_UNSUPPORTED, "bad sizes");
     StreamArgs a{};
     a.p = p;
     a.status = fg_status_word_device_ptr();
     a.rows = group_rows(p.N);
     a.groups = (int)fg_cdiv(p.N, a.rows);
-    return p.M <= 8 ? launch_rows<1>(a, st) : p.M <= 16 ? launch_rows<2>(a, st) : p.M <= 32 ? launch_rows<4>(a, st) : launch_rows<8>(a, st);
+    // A tcgen05 instruction takes 64 cycles for its 128 rows of tokens however few they are and however low the group is, 142 ns
+    // per block of K, where the registers' instructions take what tokens and rows cost; those run out above (0.4 PFLOP/s).
+    // Measured, registers / TMEM: 2112 x 7168 5.6 / 10.7 us with 16 tokens, 7.2 / 10.6 with 32; 6144 x 4096 7.6 / 8.9 with 16,
+    // 9.5 / 8.9 with 32; 24576 x 7168 33.3 / 33.1 and 39.1 / 33.2; 4096 x 14336 15.7 / 20.2 with 32, 21.8 / 19.7 with 33.
+    const bool registers = p.M <= 16 || (p.M <= 32 && a.rows <= 32);
+    return registers ? launch_registers(a, st) : launch_tensor_memory(a, st);
 }

@@ -44,12 +44,12 @@ def _check(got, pre, bias=None, rounded_before_bias=False):
     assert bool((err <= bound * 1.001).all()), (float(err.max()), float((err / bound.clamp_min(1e-300)).max()))
 
 
-# few tokens (8, 16, 32, 64 at a time; groups of 16 to 256 weight rows, one or several per CTA; K with and without whole
-# blocks of 128), split K, single and paired tiles, ragged edges in every dimension
+# few tokens (8, 16 or 32 in registers, up to 128 in TMEM; groups of 16 to 256 weight rows, one or several per CTA; K with and
+# without whole blocks of 128), single and paired tiles, ragged edges in every dimension
 SHAPES = [(1, 1, 16), (1, 256, 128), (1, 6144, 4096), (1, 2112, 7168), (1, 28672, 1024), (2, 33, 48), (3, 100003, 272), (7, 130, 2064),
           (8, 40000, 528), (9, 37889, 256), (16, 28672, 4096), (17, 75777, 384), (20, 24576, 1040), (24, 15000, 784), (31, 4096, 4096),
           (32, 300, 16), (32, 28672, 2048), (33, 208, 496), (50, 4096, 4096), (64, 9472, 208), (64, 9473, 208), (64, 24576, 1040),
-          (83, 7744, 3888), (100, 2112, 7168), (128, 4096, 14336), (129, 144, 144), (130, 4097, 528), (257, 9500, 256),
+          (65, 60000, 400), (83, 7744, 3888), (97, 37889, 128), (100, 2112, 7168), (127, 20000, 656), (128, 4096, 14336), (128, 76000, 256), (129, 144, 144), (130, 4097, 528), (257, 9500, 256),
           (1024, 6144, 4096), (1037, 6145, 4096), (4099, 8191, 512), (8192, 8192, 1024)]
 
 
@@ -68,7 +68,7 @@ def test_tiles_of_every_width(m, n):
     _check(flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, c, torch.float16), _definition(a, b, a_s, b_s), c)
 
 
-@pytest.mark.parametrize("m", [1, 20, 200])
+@pytest.mark.parametrize("m", [1, 20, 100, 200])
 @pytest.mark.parametrize("n", [4096, 30000])
 def test_operands_that_the_kernel_before_writes(m, n):
     """The product may be launched while its operands are still being written, into memory that held others before."""
@@ -86,7 +86,7 @@ def test_operands_that_the_kernel_before_writes(m, n):
         _check(c, _definition(a, b, a_s, b_s))
 
 
-@pytest.mark.parametrize("m", [1, 5, 12, 31, 60])
+@pytest.mark.parametrize("m", [1, 5, 12, 31, 60, 120])
 def test_few_tokens_twice_at_once(m):
     """The same call on two streams, and one after another without a wait between."""
     ops = [_operands(m, 20000 + 16 * i, 2048, seed=i) for i in range(4)]
@@ -104,7 +104,7 @@ def test_few_tokens_twice_at_once(m):
     assert _cabi.device_status() == 0
 
 
-@pytest.mark.parametrize("m", [1, 5, 40, 300])
+@pytest.mark.parametrize("m", [1, 5, 20, 40, 128, 300])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float16, torch.float32])
 def test_types_and_bias(m, out, bias):
@@ -153,7 +153,7 @@ def test_strides_and_alignment():
     assert torch.equal(flag_gems.w8a8_int8_matmul(a, b, a_s, every_other), want)
 
 
-@pytest.mark.parametrize("m", [1, 16, 300])
+@pytest.mark.parametrize("m", [1, 16, 100, 300])
 def test_sums_at_the_edge_of_32_bits(m):
     """K as large as it may be with every product 2^14: the largest sum is 2^31 - 2^18."""
     k = 131056
@@ -183,7 +183,7 @@ def test_special_scales():
     _check(got[keep], want[keep])
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (33, 208, 496), (700, 4096, 256)])
+@pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (33, 208, 496), (90, 9008, 512), (700, 4096, 256)])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
 def test_cutlass_scaled_mm(m, n, k, bias, out):
