@@ -354,17 +354,24 @@ __global__ void __launch_bounds__(256, 1) int8_stream_kernel(const __grid_consta
         const uint32_t idesc = umma_idesc_s8_s32(128, a.rows);
         int stage = 0;
         uint32_t phase = 0, round = 0;
-        bool ok = true;
+        bool ok = true, ready = false;  // ready: the next stage had come when it was last looked at
         for (int grp = blockIdx.x; grp < a.groups && ok; grp += gridDim.x, ++round) {
             const uint32_t buf = round & 1u, d = tmem + buf * acc_cols;
             ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((round >> 1) & 1u) ^ 1u, abort_flag, a.status, 23));
             if (!ok) break;
             tc_fence_after_sync();
             for (int step = 0; step < steps; ++step) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, a.status, 24));
+                ok = __all_sync(0xffffffffu, ready || mbar_wait(&full_bar[stage], phase, abort_flag, a.status, 24));
                 if (!ok) break;
+                uint64_t* this_empty = &empty_bar[stage];
+                const uint32_t x_addr = smem_u32(ring + (size_t)stage * stage_bytes);
+                if (++stage == a.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                ready = mbar_test_wait(&full_bar[stage], phase);  // answered while the instructions are issued
                 if (elect_one()) {
-                    const uint32_t x_addr = smem_u32(ring + (size_t)stage * stage_bytes), w_addr = x_addr + KB * x_block;
+                    const uint32_t w_addr = x_addr + KB * x_block;
 #pragma unroll
                     for (int b = 0; b < KB; ++b) {
                         const uint64_t x_desc = umma_desc_k_sw128(x_addr + b * x_block), w_desc = umma_desc_k_sw128(w_addr + b * w_block);
@@ -372,14 +379,10 @@ __global__ void __launch_bounds__(256, 1) int8_stream_kernel(const __grid_consta
                         for (int k = 0; k < BLOCK_K / 32; ++k)
                             umma_i8(d, x_desc + (uint64_t)(2 * k), w_desc + (uint64_t)(2 * k), idesc, step > 0 || b > 0 || k > 0 ? 1u : 0u);
                     }
-                    umma_commit(&empty_bar[stage]);
+                    umma_commit(this_empty);
                     if (step == steps - 1) umma_commit(&acc_full[buf]);
                 }
                 __syncwarp();
-                if (++stage == a.stages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
             }
         }
     } else if (warp >= 4) {
