@@ -70,6 +70,7 @@ struct FgGroupedGemm {
     int operand;  // 0 e4m3, 1 int8, 2 bf16, 3 fp16
     int block_rows, scale_mode, a_scale_per_row, fuse_silu, scatter, mul_weight, out_dtype;
     int cta_pairs;  // block_rows = 256: every block is one tile row of a CTA pair
+    int tile_width;  // int8 without SiLU: columns of a tile (0: 128 or 256 by the number of tiles)
     const float* bias;  // fp32, added before the cast; bias_stride elements between the rows of consecutive experts
     int64_t bias_stride;
     const int32_t* dest;
@@ -91,6 +92,14 @@ struct FgSkinny {
 };
 bool fg_int8_is_skinny(int64_t M);
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st);
+
+// Tile of an int8 product: its width and kind (one CTA per 128 rows, or a CTA pair per 256) with the least estimated
+// time, for so many blocks of rows of either kind (blocks256 0: no pairs) and tiles of at least `narrowest` columns.
+struct FgInt8Tile {
+    bool pair;
+    int width;
+};
+FgInt8Tile fg_int8_tile(int64_t blocks128, int64_t blocks256, int64_t N, int64_t K, int narrowest);
 
 // The rows of a grouped product's result that follow its last group, to be filled with zeros (c NULL: left as they are).
 struct FgTail {

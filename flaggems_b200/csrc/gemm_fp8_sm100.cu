@@ -1358,36 +1358,6 @@ int launch_inst(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& 
     return FG_OK;
 }
 
-// Tile of a dense int8 product of more than 128 rows: the width and the kind (one CTA per 128 rows, or a CTA pair per
-// 256) with the least estimated time.  That is the number of waves of tiles times what a block of K takes, which hardly
-// depends on the width below 256 (the ring's round trip; above, the 64 bytes per cycle that an SM takes in).  So a narrower
-// tile pays where it saves a wave, and a pair where a tile's K is long enough for its dearer start.  The constants (ns) are
-// fitted to 5 weights x 12 row counts x 11 tiles; the choices are within 6 % of the best of the 11.  Measured, 256-wide
-// single / 256-wide pair / this: 1037 x 6144 x 4096 32.3 / 28.7 / 27.0 us (pairs of 224 columns, two full waves),
-// 300 x 7168 x 2048 13.3 / 13.2 / 12.0 (single, 160), 777 x 4096 x 14336 51.1 / 44.1 / 44.1, 1037 x 4096 x 14336 52.3 /
-// 75.0 / 52.3, 256 x 6144 x 4096 19.6 / 17.5 / 15.4 (single, 96).
-struct Int8Tile {
-    bool pair;
-    int width;
-};
-Int8Tile int8_tile(int64_t M, int64_t N, int64_t k_blocks, int sms) {
-    Int8Tile best{false, 256};
-    int64_t least = INT64_MAX;
-    auto offer = [&](bool pair, int width, int64_t start, int64_t per_block) {
-        const int64_t tiles = fg_cdiv(M, pair ? 2 * BLOCK_M : BLOCK_M) * fg_cdiv(N, width);
-        const int64_t time = start + fg_cdiv(tiles, pair ? sms / 2 : sms) * k_blocks * per_block;
-        if (time < least) {
-            least = time;
-            best = Int8Tile{pair, width};
-        }
-    };
-    for (int width = 256; width >= 96; width -= 32) offer(false, width, 4000, 290 + 130 * width / 256);
-    offer(false, 64, 4000, 285);
-    if (pair_enabled())
-        for (int width = 256; width >= 128; width -= 32) offer(true, width, 5500, 265 + 80 * width / 256);
-    return best;
-}
-
 // Rows of both operands in bytes.
 int check_operands(const void* a, const void* b, int64_t K, int64_t ld_a, int64_t ld_b) {
     FG_REQUIRE(K > 0 && K % 16 == 0, FG_ERR_UNSUPPORTED, "K = %d must be a positive multiple of 16", (int)K);
@@ -1398,7 +1368,7 @@ int check_operands(const void* a, const void* b, int64_t K, int64_t ld_a, int64_
 }
 
 int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, const void* b, int num_experts,
-                int64_t ld_b, bool block_scaled, bool fuse_silu, cudaStream_t st) {
+                int64_t ld_b, bool block_scaled, bool fuse_silu, cudaStream_t st, int want_width = 0) {
     const int operands_rc = check_operands(a, b, p.K, ld_a, ld_b);
     if (operands_rc != FG_OK) return operands_rc;
     p.status = fg_status_word_device_ptr();
@@ -1457,10 +1427,13 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     p.tile_n = fuse_silu ? bn / 2 : bn;
     bool int8_pair = false;
     if (p.int8 == 1 && !p.grouped) {
-        const Int8Tile t = int8_tile(p.M, p.n_out, fg_cdiv(p.K, BLOCK_K), sms);
+        const FgInt8Tile t = fg_int8_tile(fg_cdiv(p.M, BLOCK_M), fg_cdiv(p.M, 2 * BLOCK_M), p.n_out, p.K, 64);
         int8_pair = t.pair;
-        p.tile_n = t.width;
         bn = t.width > 128 || t.pair ? 256 : t.width > 64 ? 128 : 64;
+        p.tile_n = t.width;
+    } else if (want_width > 0) {
+        bn = want_width > 128 || grouped_pair ? 256 : 128;
+        p.tile_n = want_width;
     }
     const int64_t pair_tiles = fg_cdiv(p.M, 2 * BLOCK_M) * fg_cdiv(p.n_out, fuse_silu ? 128 : int8_pair ? p.tile_n : 256);
     const bool pair = int8_pair || grouped_pair || (p.int8 == 0 && !p.grouped && !fuse_silu && !block_scaled && bn == 256 && k_slices == 1 &&
@@ -1679,6 +1652,33 @@ int fg_grouped_gemm_fp8_bias(void* c, const void* a, const void* w, const float*
 
 }  // extern "C"
 
+// The estimate is the number of waves of tiles times what a block of K takes, which hardly depends on the width below 256
+// (the ring's round trip; above, the 64 bytes per cycle that an SM takes in).  So a narrower tile pays where it saves a
+// wave, and a pair where a tile's K is long enough for its dearer start.  The constants (ns) are fitted to 5 weights x 12 row
+// counts x 11 tiles; the choices are within 6 % of the best of the 11.  Measured, 256-wide single / 256-wide pair / this:
+// 1037 x 6144 x 4096 32.3 / 28.7 / 27.0 us (pairs of 224 columns, two full waves), 300 x 7168 x 2048 13.3 / 13.2 / 12.0
+// (single, 160), 777 x 4096 x 14336 51.1 / 44.1 / 44.1, 1037 x 4096 x 14336 52.3 / 75.0 / 52.3, 256 x 6144 x 4096 19.6 /
+// 17.5 / 15.4 (single, 96).
+FgInt8Tile fg_int8_tile(int64_t blocks128, int64_t blocks256, int64_t N, int64_t K, int narrowest) {
+    const int sms = fg_num_sms();
+    const int64_t k_blocks = fg_cdiv(K, BLOCK_K);
+    FgInt8Tile best{false, 256};
+    int64_t least = INT64_MAX;
+    auto offer = [&](bool pair, int width, int64_t start, int64_t per_block) {
+        const int64_t tiles = (pair ? blocks256 : blocks128) * fg_cdiv(N, width);
+        const int64_t time = start + fg_cdiv(tiles, pair ? sms / 2 : sms) * k_blocks * per_block;
+        if (time < least) {
+            least = time;
+            best = FgInt8Tile{pair, width};
+        }
+    };
+    for (int width = 256; width >= 96; width -= 32) offer(false, width, 4000, 290 + 130 * width / 256);
+    if (narrowest <= 64) offer(false, 64, 4000, 285);
+    if (blocks256 > 0 && pair_enabled())
+        for (int width = 256; width >= 128; width -= 32) offer(true, width, 5500, 265 + 80 * width / 256);
+    return best;
+}
+
 int fg_grouped_gemm(const FgGroupedGemm& g, cudaStream_t stream) {
     FG_REQUIRE(g.max_rows >= 0 && g.N > 0 && g.K > 0 && g.num_experts > 0, FG_ERR_INVALID_ARGUMENT, "bad sizes");
     FG_REQUIRE((g.c || g.n_peers > 0) && g.a && g.w && g.a_scale && g.w_scale && g.sorted_ids && g.expert_ids && g.num_post_pad,
@@ -1729,7 +1729,8 @@ int fg_grouped_gemm(const FgGroupedGemm& g, cudaStream_t stream) {
     p.dest = g.dest; p.dest_stride = g.dest_stride; p.n_peers = g.n_peers; p.peer_rows = g.peer_rows;
     for (int i = 0; i < g.n_peers; ++i) p.peer_out[i] = g.peer_out[i];
     if (g.n_peers > 0 && !g.c) p.c = g.peer_out[0];
-    return launch_gemm(p, g.a, g.gather_div > 0 ? g.a_rows : p.M, ld_a, g.w, g.num_experts, K, block, g.fuse_silu != 0, stream);
+    return launch_gemm(p, g.a, g.gather_div > 0 ? g.a_rows : p.M, ld_a, g.w, g.num_experts, K, block, g.fuse_silu != 0, stream,
+                       g.operand == 1 && !g.fuse_silu ? g.tile_width : 0);
 }
 
 // The C-ABI forms: rows of a in sorted order.

@@ -26,6 +26,7 @@ namespace {
 constexpr int TILE_ROWS = 128;
 constexpr int PAIR_ROWS = 256;      // rows of a CTA pair's tile
 constexpr int PAIR_MIN_ROWS = 768;  // rows per expert from which pairs are used (see use_pairs)
+constexpr int INT8_PAIR_MIN_ROWS = 192;  // the same for int8 grouped products, which weigh the two kinds of tiles
 
 inline int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
@@ -253,7 +254,20 @@ int scaled_grouped_mm(int operand, void* c, const void* a, const void* b, const 
     FG_REQUIRE(c && a && b && scale_a && scale_b && offs && workspace, FG_ERR_INVALID_ARGUMENT, "null pointer");
     FG_REQUIRE((uintptr_t)workspace % 256 == 0, FG_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
     FG_REQUIRE(ld_a % 16 == 0 && (uintptr_t)a % 16 == 0, FG_ERR_UNSUPPORTED, "a must have 16-byte aligned rows");
-    const bool pairs = use_pairs(m_total, num_groups, N, N);
+    bool pairs = use_pairs(m_total, num_groups, N, N);
+    int width = 0;
+    // int8: by the estimate for tiles, where the rows of a group make up for its weight or a few waves of tiles are all there
+    // is.  In between the weights' stream decides, and the plain rule does better.  Estimate / plain rule, 8 groups: 2048 x
+    // 4096 x 14336 161 / 184 us, 6000 x 4096 x 14336 277 / 306, 6000 x 28672 x 4096 538 / 599; but 2048 x 28672 x 4096 302 / 271,
+    // and 1536 x 4096 x 7168 in 32 groups 175 / 163.
+    const int64_t blocks = m_total / TILE_ROWS + (num_groups + 1) / 2;  // a group ends half a block before its last block, on average
+    const bool few_waves = m_total >= 96 * (int64_t)num_groups && blocks * fg_cdiv(N, 256) <= 4 * (int64_t)fg_num_sms();
+    if (operand == 1 && (few_waves || m_total >= 448 * (int64_t)num_groups)) {
+        const bool enough = m_total >= INT8_PAIR_MIN_ROWS * (int64_t)num_groups;
+        const FgInt8Tile t = fg_int8_tile(blocks, enough ? m_total / PAIR_ROWS + (num_groups + 1) / 2 : 0, N, K, 128);
+        pairs = t.pair;
+        width = t.width;
+    }
     const int tile = pairs ? PAIR_ROWS : TILE_ROWS;
     const Workspace ws = carve_grouped_mm(workspace, m_total, num_groups, tile);
     FG_REQUIRE(workspace_bytes >= ws.bytes, FG_ERR_INVALID_ARGUMENT, "workspace holds %lld bytes, needs %lld",
@@ -264,7 +278,7 @@ int scaled_grouped_mm(int operand, void* c, const void* a, const void* b, const 
                             ws.post_pad, tail, st);
     if (rc != FG_OK) return rc;
     FgGroupedGemm g{};
-    g.operand = operand;
+    g.operand = operand; g.tile_width = width;
     g.sorted_ids = ws.sorted_ids; g.expert_ids = ws.expert_ids; g.num_post_pad = ws.post_pad; g.max_rows = ws.rows;
     g.numel = m_total; g.num_experts = num_groups; g.block_rows = tile; g.cta_pairs = pairs; g.scale_mode = FG_SCALE_VECTOR; g.out_dtype = out_dtype;
     g.c = c; g.a = a; g.w = b; g.a_scale = scale_a; g.w_scale = scale_b; g.bias = bias; g.bias_stride = bias_stride_g;
@@ -282,7 +296,7 @@ int64_t fg_scaled_grouped_mm_workspace_bytes(int64_t m_total, int num_groups, in
     // The larger of the tables that the call may choose: its N is not known here.  Tables of 256-row blocks hold more
     // padding, those of 128-row blocks more block ids (the larger part above ~32768 rows per group).
     const int64_t single = carve_grouped_mm(nullptr, m_total, num_groups, TILE_ROWS).bytes;
-    if (m_total < PAIR_MIN_ROWS * (int64_t)num_groups) return single;
+    if (m_total < INT8_PAIR_MIN_ROWS * (int64_t)num_groups) return single;
     const int64_t paired = carve_grouped_mm(nullptr, m_total, num_groups, PAIR_ROWS).bytes;
     return single > paired ? single : paired;
 }

@@ -236,6 +236,19 @@ def test_grouped(sizes, n, k):
     _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs), _grouped_definition(a, b, a_s, b_s, offs))
 
 
+@pytest.mark.parametrize("sizes", [[700, 0, 130, 400], [100, 250, 97, 3, 300], [1300, 700, 900], [2100, 1500]], ids=str)
+@pytest.mark.parametrize("n", [2112, 4096, 6200])
+def test_grouped_tiles_of_every_width(sizes, n):
+    a, b, a_s, b_s, offs, g = _grouped(sizes, n, 2064, seed=n, tail=5)
+    bias = torch.randn(len(sizes), n, device="cuda", generator=g)
+    want = _grouped_definition(a, b, a_s, b_s, offs)
+    _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs), want)
+    group = torch.repeat_interleave(torch.arange(len(sizes), device="cuda"), torch.tensor(sizes, device="cuda"))
+    got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs, bias, torch.float16)
+    _check(got[:-5], want[:-5], bias[group])
+    assert not got[-5:].any()
+
+
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("tail", [1, 200])
 @pytest.mark.parametrize("n", [64, 65])
