@@ -316,6 +316,9 @@ PyObject* scaled_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
         if (!c || !a || !b || !sa || !sb || a->scalar_type() != b->scalar_type()) return none();
         const bool int8 = cutlass && a->scalar_type() == ScalarType::Char;  // aten _scaled_mm has no int8 operands
         if (!int8 && a->scalar_type() != E4M3) return none();
+        if (int8)
+            for (const at::Tensor* t : {c, b, sa, sb})
+                if (t->device() != a->device()) return none();
         if (a->dim() != 2 || b->dim() != 2 || c->dim() != 2) return none();
         const int64_t m = a->size(0), k = a->size(1), cols = b->size(1);
         const int code = c->scalar_type() == E4M3 ? FG_DTYPE_E4M3 : dtype_code(c->scalar_type());
@@ -333,6 +336,7 @@ PyObject* scaled_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
             bias = cuda_tensor(p[5]);
             const ScalarType want = code == FG_DTYPE_E4M3 ? ScalarType::Float : c->scalar_type();
             if (!bias || bias->scalar_type() != want || bias->dim() != 1 || bias->size(0) != cols || !bias->is_contiguous()) return none();
+            if (int8 && bias->device() != a->device()) return none();
         }
         const int rc = unlocked([&] {
             c10::cuda::CUDAGuard guard(a->device());

@@ -52,6 +52,9 @@ def cutlass_scaled_mm(
     int8 = a.dtype == torch.int8
     if a.dtype != b.dtype or not (int8 or a.dtype == torch.float8_e4m3fn):
         raise AssertionError(f"Unsupported dtype: {a.dtype} and {b.dtype}")
+    if int8:
+        for t in (c, b, a_scale, b_scale, bias):
+            assert t is None or t.device == a.device, f"operands on {a.device} and {t.device}"
     if c.dtype not in _cabi.DTYPE_CODE:
         raise NotImplementedError(f"unsupported output dtype {c.dtype}")
     L = _cabi.lib()

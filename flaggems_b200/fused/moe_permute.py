@@ -146,6 +146,7 @@ def moe_permute(
         raise NotImplementedError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     if hidden_states.dtype not in _ELEMENT_BYTES:
         raise NotImplementedError(f"unsupported dtype {hidden_states.dtype}")
+    num_experts = int(num_experts)
     assert num_experts > 0, "num_experts must be positive"
     x = _rows(hidden_states, "hidden_states")
     assert x.shape[0] == topk_ids.shape[0], f"{x.shape[0]} tokens, {topk_ids.shape[0]} rows of topk_ids"

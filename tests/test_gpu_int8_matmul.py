@@ -166,6 +166,19 @@ def test_sums_at_the_edge_of_32_bits(m):
     assert torch.equal(got, want.double().float())
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 3000017, 128), (12, 9000000, 16), (128, 17000000, 16), (40000, 55000, 64)])
+def test_many_groups_and_outputs_past_32_bits(m, n, k):
+    """Thousands of groups of weight rows per CTA; up to 2.2e9 outputs (4.4 GB)."""
+    a, b, a_s, b_s, g = _operands(m, n, k)
+    got = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s)
+    assert got.shape == (m, n)
+    at = torch.cat([torch.arange(700, device="cuda"), torch.randint(0, n, (4000,), device="cuda", generator=g),
+                    torch.arange(n - 700, n, device="cuda")])
+    rows = torch.tensor(sorted({0, m // 3, m - 1}), device="cuda")
+    _check(got[rows][:, at], _definition(a[rows], b[at], a_s[rows], b_s[at]))
+    assert _cabi.device_status() == 0
+
+
 def test_nothing_to_compute():
     one = torch.ones(1, device="cuda")
     a, b = torch.zeros(0, 64, dtype=I8, device="cuda"), torch.zeros(32, 64, dtype=I8, device="cuda")
