@@ -662,6 +662,15 @@ at::Tensor unpermuted(const at::Tensor& rows, const at::Tensor& row_of_slot, con
     return out;
 }
 
+// A contiguous part of a one-dimensional tensor, from value `first` on, seen with other sizes.  What as_strided returns, in a
+// tenth of its time; the parts of one allocation do not overlap.
+at::Tensor part_of(const at::Tensor& t, int64_t first, at::IntArrayRef sizes) {
+    at::Tensor p = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+    p.unsafeGetTensorImpl()->set_storage_offset(first);
+    p.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return p;
+}
+
 struct Permuted {
     at::Tensor rows, row_scale, offs, row_of_slot, slot_of_row;
 };
@@ -672,9 +681,10 @@ Permuted permuted(const at::Tensor& x, const at::Tensor& ids, int64_t experts, c
     Permuted p;
     p.rows = empty({n, x.size(1)}, x.scalar_type(), x);
     if (scale) p.row_scale = empty({n, cols}, ScalarType::Float, x);
-    p.offs = empty({experts}, ScalarType::Int, x);
-    p.row_of_slot = empty({tokens, topk}, ScalarType::Int, x);
-    p.slot_of_row = empty({n}, ScalarType::Int, x);
+    const at::Tensor ints = empty({2 * n + experts}, ScalarType::Int, x);
+    p.row_of_slot = part_of(ints, 0, {tokens, topk});
+    p.slot_of_row = part_of(ints, n, {n});
+    p.offs = part_of(ints, 2 * n, {experts});
     const int64_t need = std::max<int64_t>(fg_moe_permute_workspace_bytes(tokens, (int)topk, (int)experts), 0);
     const at::Tensor ws = need ? empty({need}, ScalarType::Byte, x) : at::Tensor();
     throw_rc(fg_moe_permute(p.rows.data_ptr(), scale ? static_cast<float*>(p.row_scale.data_ptr()) : nullptr,

@@ -233,18 +233,18 @@ __global__ void __launch_bounds__(256) permute_rows_kernel(SortArgs s, ChunkTabl
 
 // Few slots: sorting and copying in one launch.  The CTA of a token counts for each of its slots the slots that come
 // before it in (expert, slot) order, which is the slot's row, while the token's row is on its way.  The last
-// CTA counts the experts instead.
-template <typename UNIT>
+// CTA counts the experts instead.  With few tokens each has several CTAs, for a part of its row each (blockIdx.y).
+template <typename UNIT, int PIECES>
 __global__ void __launch_bounds__(256) sort_and_permute_kernel(SortArgs s, RowArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
-    constexpr int PIECES = 4;
     __shared__ int32_t hist[MAX_EXPERTS];
     __shared__ int32_t before[8][SLOTS_AT_ONCE];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int numel = (int)s.numel, E = s.num_experts;
     const int64_t t = blockIdx.x;
     if (t * a.topk >= numel) {
+        if (blockIdx.y > 0) return;
         for (int e = threadIdx.x; e < E; e += blockDim.x) hist[e] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < numel; i += blockDim.x) {
@@ -252,23 +252,30 @@ __global__ void __launch_bounds__(256) sort_and_permute_kernel(SortArgs s, RowAr
             if (e < E) atomicAdd(&hist[e], 1);
         }
         __syncthreads();
-        if (warp == 0) {
-            int32_t run = 0;
-            for (int e0 = 0; e0 < E; e0 += 32) {
-                int32_t incl = e0 + lane < E ? hist[e0 + lane] : 0;
+        int32_t run = 0;
+        for (int e0 = 0; e0 < E; e0 += blockDim.x) {
+            const int e = e0 + (int)threadIdx.x;
+            int32_t incl = e < E ? hist[e] : 0;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += v;
-                }
-                if (e0 + lane < E) s.offs[e0 + lane] = run + incl;
-                run += __shfl_sync(0xffffffffu, incl, 31);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
             }
+            if (lane == 31) before[warp][0] = incl;
+            __syncthreads();
+            int32_t all = 0;
+            for (int w = 0; w < warps; ++w) {
+                if (w < warp) incl += before[w][0];
+                all += before[w][0];
+            }
+            if (e < E) s.offs[e] = run + incl;
+            run += all;
+            __syncthreads();
         }
         return;
     }
     UNIT piece[PIECES];
-    const int v0 = threadIdx.x;
+    const int v0 = blockIdx.y * PIECES * blockDim.x + threadIdx.x;
     load_pieces(a, t, v0, piece);
     for (int k0 = 0; k0 < a.topk; k0 += SLOTS_AT_ONCE) {
         const int first = (int)t * a.topk + k0;
@@ -298,18 +305,18 @@ __global__ void __launch_bounds__(256) sort_and_permute_kernel(SortArgs s, RowAr
             for (int w = 0; w < warps; ++w) r[k] += before[w][k];
             if (k0 + k >= a.topk) continue;
             const bool none = key[k] >= E * numel;
-            if (threadIdx.x == 0) {
+            if (threadIdx.x == 0 && blockIdx.y == 0) {
                 s.slot_of_row[r[k]] = first + k;
                 s.row_of_slot[first + k] = none ? ~r[k] : r[k];
             }
             if (none) r[k] = ~r[k];
             store_pieces(a, r[k], v0, piece);
-            for (int v = v0 + PIECES * blockDim.x; v < a.units; v += PIECES * blockDim.x) {  // rows of more than 16 KB
+            for (int v = v0 + gridDim.y * PIECES * blockDim.x; v < a.units; v += gridDim.y * PIECES * blockDim.x) {
                 UNIT more[PIECES];
                 load_pieces(a, t, v, more);
                 store_pieces(a, r[k], v, more);
             }
-            if (a.scale_cols) store_scales(a, t, k0 + k, r[k]);
+            if (a.scale_cols && blockIdx.y == 0) store_scales(a, t, k0 + k, r[k]);
         }
         __syncthreads();
     }
@@ -596,7 +603,16 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
         return vec ? go(uint4()) : elem_bytes == 4 ? go((unsigned int)0) : elem_bytes == 2 ? go((unsigned short)0) : go((unsigned char)0);
     };
     if (numel > 0 && one_launch(T, numel, row_bytes)) {
-        FG_CUDA(by_unit([&](auto u) { return fg_launch(sort_and_permute_kernel<decltype(u)>, (unsigned)T + 1, threads < 128 ? 128u : threads, 0, st, 1, a, r); }));
+        // A row per CTA, four pieces per thread; with few tokens two pieces, and parts of a row until there are two CTAs per SM.
+        const unsigned block = threads < 128 ? 128u : threads;
+        unsigned parts = 1;
+        while (parts < 32 && T * parts * 2 <= 2 * fg_num_sms() && parts * 2 * block < (unsigned)r.units) parts *= 2;
+        const dim3 grid((unsigned)T + 1, parts);
+        FG_CUDA(by_unit([&](auto u) {
+            using U = decltype(u);
+            return parts > 1 ? fg_launch(sort_and_permute_kernel<U, 2>, grid, block, 0, st, 1, a, r)
+                             : fg_launch(sort_and_permute_kernel<U, 4>, grid, block, 0, st, 1, a, r);
+        }));
         return FG_OK;
     }
     if (numel == 0) {
