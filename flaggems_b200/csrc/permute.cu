@@ -136,13 +136,36 @@ struct RowArgs {
 };
 constexpr int SLOTS_AT_ONCE = 8;
 
+struct __align__(32) Unit32 {
+    uint4 lo, hi;
+};
+
+template <typename UNIT>
+__device__ __forceinline__ UNIT load_unit(const UNIT* p) { return *p; }
+template <>
+__device__ __forceinline__ Unit32 load_unit(const Unit32* p) {
+    Unit32 v;
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v.lo.x), "=r"(v.lo.y), "=r"(v.lo.z), "=r"(v.lo.w), "=r"(v.hi.x), "=r"(v.hi.y), "=r"(v.hi.z), "=r"(v.hi.w)
+                 : "l"(p) : "memory");
+    return v;
+}
+template <typename UNIT>
+__device__ __forceinline__ void store_unit(UNIT* p, const UNIT& v) { *p = v; }
+template <>
+__device__ __forceinline__ void store_unit(Unit32* p, const Unit32& v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(v.lo.x), "r"(v.lo.y), "r"(v.lo.z), "r"(v.lo.w), "r"(v.hi.x), "r"(v.hi.y), "r"(v.hi.z), "r"(v.hi.w)
+                 : "memory");
+}
+
 template <typename UNIT, int N>
 __device__ __forceinline__ void load_pieces(const RowArgs& a, int64_t t, int v0, UNIT (&piece)[N]) {
     const UNIT* x = reinterpret_cast<const UNIT*>(a.x) + t * a.ld_x;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int v = v0 + u * (int)blockDim.x;
-        piece[u] = v < a.units ? x[v] : UNIT{};
+        piece[u] = v < a.units ? load_unit(x + v) : UNIT{};
     }
 }
 
@@ -154,7 +177,7 @@ __device__ __forceinline__ void store_pieces(const RowArgs& a, int32_t r, int v0
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int v = v0 + u * (int)blockDim.x;
-        if (v < a.units) out[v] = r < 0 ? UNIT{} : piece[u];
+        if (v < a.units) store_unit(out + v, r < 0 ? UNIT{} : piece[u]);
     }
 }
 
@@ -196,16 +219,17 @@ __global__ void __launch_bounds__(256) scan_chunks_kernel(SortArgs s, ChunkTable
     }
 }
 
-// Many slots, third launch, one CTA per token: its row is read once, two pieces per thread, and written slot after
-// slot.  Bound by the writes, which are topk times the reads.  Few registers (and so many CTAs, a row each, under way)
-// matter more than pieces per thread: 8192 x 8 rows of 7168 bytes take 88 us this way, 98 with four pieces and the slots'
-// rows in registers, 91-97 as bulk copies through a ring in shared memory (6.0 TB/s of the 6.6 of a copy).
-// UNIT: the bytes of a load, 16 where everything is aligned to that.
+// Many slots, third launch, one CTA per token: its row is read once and written slot after slot.  Bound by the writes, which
+// are topk times the reads, and by the rate of a copy.  Few registers (and so many CTAs, a row each, under way) matter more
+// than pieces per thread, and accesses of 32 bytes more than those of 16: 8192 x 8 rows of 14336 bytes take 164 us (6.4 TB/s
+// of the 6.6 of a copy), 178 with two pieces of 16 bytes per thread; rows of 7168 bytes 84, 88, and 98 with four pieces and the
+// slots' rows in registers, 91-97 as bulk copies through a ring in shared memory.
+// UNIT: the bytes of a load, 32 or 16 where everything is aligned to that.
 template <typename UNIT>
-__global__ void __launch_bounds__(256) permute_rows_kernel(SortArgs s, ChunkTable ct, RowArgs a) {
+__global__ void __launch_bounds__(512) permute_rows_kernel(SortArgs s, ChunkTable ct, RowArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
-    constexpr int PIECES = 2, SLOTS = 32;
+    constexpr int PIECES = sizeof(UNIT) == 32 ? 1 : 2, SLOTS = 32;
     __shared__ int32_t row_s[SLOTS];
     const int64_t t = blockIdx.x;
     UNIT piece[PIECES];
@@ -595,9 +619,12 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
     cudaStream_t st = (cudaStream_t)stream;
     const SortArgs a{topk_ids, ids_are_i64, numel, num_experts, expert_map, expert_map_len, offs, row_of_slot, slot_of_row};
     const int64_t row_bytes = H * elem_bytes;
-    const bool vec = aligned16(x, ld_x * elem_bytes) && aligned16(rows, row_bytes);
-    const int unit = vec ? 16 : elem_bytes;
-    const RowArgs r{x, ld_x * elem_bytes / unit, scale, ld_scale, topk, numel, rows, (int)(row_bytes / unit), row_scale, (int)scale_cols};
+    const auto aligned = [&](int to) { return (uintptr_t)x % to == 0 && (uintptr_t)rows % to == 0 && ld_x * elem_bytes % to == 0 && row_bytes % to == 0; };
+    const bool vec = aligned(16);
+    const auto row_args = [&](int unit) {
+        return RowArgs{x, ld_x * elem_bytes / unit, scale, ld_scale, topk, numel, rows, (int)(row_bytes / unit), row_scale, (int)scale_cols};
+    };
+    const RowArgs r = row_args(vec ? 16 : elem_bytes);
     const unsigned threads = threads_for(r.units);
     auto by_unit = [&](auto&& go) -> cudaError_t {
         return vec ? go(uint4()) : elem_bytes == 4 ? go((unsigned int)0) : elem_bytes == 2 ? go((unsigned short)0) : go((unsigned char)0);
@@ -625,7 +652,15 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
     const ChunkTable ct = chunk_table(workspace, numel);
     const int rc = rank_slots(a, ct, st);
     if (rc != FG_OK) return rc;
-    FG_CUDA(by_unit([&](auto u) { return fg_launch(permute_rows_kernel<decltype(u)>, (unsigned)T, threads, 0, st, 1, a, ct, r); }));
+    // Early whatever the size of the grid: what it waits for is the scan alone, 3 us (fg_launch keeps grids that fill the chip
+    // back because they may wait long, in the way of other streams).
+    if (aligned(32)) {
+        const RowArgs wide = row_args(32);
+        const unsigned block = wide.units >= 512 ? 512u : wide.units <= 32 ? 32u : (unsigned)(wide.units + 31) / 32 * 32;
+        FG_CUDA(fg_launch_when(true, permute_rows_kernel<Unit32>, (unsigned)T, block, 0, st, 1, a, ct, wide));
+        return FG_OK;
+    }
+    FG_CUDA(by_unit([&](auto u) { return fg_launch_when(true, permute_rows_kernel<decltype(u)>, (unsigned)T, threads, 0, st, 1, a, ct, r); }));
     return FG_OK;
 }
 
