@@ -92,6 +92,10 @@ struct FgSkinny {
 };
 bool fg_int8_is_skinny(int64_t M);
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st);
+// The same with rows [offs[e - 1], offs[e]) of a times weight e of b [n_experts, N, K]; rows of c from offs[n_experts - 1] on
+// become zeros.  sa [M], sb [n_experts, N], bias rows bias_stride apart.
+bool fg_int8_is_skinny_grouped(int64_t M, int64_t N, int n_experts);
+int fg_int8_skinny_grouped(const FgSkinny& p, const int32_t* offs, int n_experts, int64_t bias_stride, cudaStream_t st);
 
 // Tile of an int8 product: its width and kind (one CTA per 128 rows, or a CTA pair per 256) with the least estimated
 // time, for so many blocks of rows of either kind (blocks256 0: no pairs) and tiles of at least `narrowest` columns.

@@ -45,6 +45,11 @@ struct StreamArgs {
     int stages;
     int token_rows;  // int8_stream_kernel: rows of the tokens' box, a multiple of 8
     int wide;  // one load brings all KB blocks of a stage (K a multiple of 128); otherwise each has its own
+    // Grouped (int8_skinny_kernel): p.b holds n_experts weights of p.N rows, rows [offs[e - 1], offs[e]) of p.a are expert e's,
+    // and an item of work is a group of weight rows of an expert that has rows; groups counts those of one weight.
+    const int32_t* offs;
+    int n_experts;
+    int64_t bias_stride;  // values between the bias rows of consecutive experts (0: one row)
     unsigned int* status;
 };
 
@@ -121,9 +126,51 @@ __device__ __forceinline__ void store_row(const FgSkinny& p, int64_t m, int64_t 
     }
 }
 
+// The experts that have rows (up to MOST), in order, into shared memory; returns their number.  Every CTA finds the same.
+template <int MOST>
+__device__ int experts_with_rows(const int32_t* offs, int n_experts, int rows, int (&id)[MOST], int (&first)[MOST], int (&count)[MOST],
+                                 int (&warp_count)[WARPS + 1]) {
+    constexpr int EACH = 4;  // experts per lane: up to 1024 by eight warps
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int lo[EACH], n[EACH];
+    unsigned have[EACH];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int e = (warp * EACH + i) * 32 + lane;
+        const bool in = warp < WARPS && e < n_experts;
+        lo[i] = in && e > 0 ? min(max(offs[e - 1], 0), rows) : 0;
+        n[i] = in ? min(offs[e], rows) - lo[i] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        have[i] = __ballot_sync(0xffffffffu, n[i] > 0);
+        mine += __popc(have[i]);
+    }
+    if (lane == 0) warp_count[warp] = mine;
+    __syncthreads();
+    int at = 0, all = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) at += warp_count[w];
+        all += warp_count[w];
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int to = at + __popc(have[i] & ((1u << lane) - 1u));
+        if (n[i] > 0 && to < MOST) {
+            id[to] = (warp * EACH + i) * 32 + lane;
+            first[to] = lo[i];
+            count[to] = n[i];
+        }
+        at += __popc(have[i]);
+    }
+    __syncthreads();
+    return min(all, MOST);
+}
+
 // NT: tiles of eight tokens.  KB: blocks of K per stage; 8 / KB warps share the strips of 16 rows of a block, up to SPW
 // each.  Every warp passes every stage, in order.
-template <int NT, int SPW, int KB>
+template <int NT, int SPW, int KB, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w,
                                                                  const __grid_constant__ CUtensorMap tm_x, const StreamArgs a) {
     constexpr int TOKENS = 8 * NT, WS = WARPS / KB;
@@ -138,10 +185,9 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
     int* sums = reinterpret_cast<int*>(ring + (size_t)a.stages * stage_bytes);  // [TOKENS][rows]
     volatile uint32_t* abort_flag = &abort_word;
     const int steps = ((int)p.K + KB * BLOCK_K - 1) / (KB * BLOCK_K);  // stages per group
-    if (warp == WARPS && lane == 0) {
+    if (!GROUPED && a.wide && warp == WARPS && lane == 0) {
         // While the kernel before this one drains, the first stages of the weight come as far as L2.
-        if (a.wide)
-            for (int step = 0; step < min(a.stages, steps); ++step) tma_prefetch_3d(&tm_w, 0, blockIdx.x * a.rows, step * KB);
+        for (int step = 0; step < min(a.stages, steps); ++step) tma_prefetch_3d(&tm_w, 0, blockIdx.x * a.rows, step * KB);
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
@@ -156,26 +202,31 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
     for (int i = threadIdx.x; i < TOKENS * a.rows; i += THREADS) sums[i] = 0;
     __syncthreads();
     fg_pdl_wait();
+    __shared__ int ex_id[TOKENS], ex_first[TOKENS], ex_count[TOKENS], warp_count[WARPS + 1];
+    int items = a.groups;
+    if constexpr (GROUPED) items *= experts_with_rows(a.offs, a.n_experts, (int)p.M, ex_id, ex_first, ex_count, warp_count);
 
     if (warp == WARPS) {
         if (lane == 0) {
             int stage = 0, issued = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int grp = blockIdx.x; grp < a.groups && ok; grp += gridDim.x)
+            for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+                const int ex = GROUPED ? item / a.groups : 0;
+                const int w_row = GROUPED ? ex_id[ex] * (int)p.N + item % a.groups * a.rows : item * a.rows, x_row = GROUPED ? ex_first[ex] : 0;
                 for (int step = 0; step < steps; ++step) {
                     ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, a.status, 20);
                     if (!ok) break;
                     uint8_t* to = ring + (size_t)stage * stage_bytes;
                     mbar_arrive_expect_tx(&full_bar[stage], (uint32_t)stage_bytes);
                     if (a.wide) {
-                        tma_load_3d(to, &tm_w, &full_bar[stage], 0, grp * a.rows, step * KB);
-                        tma_load_3d(to + w_bytes, &tm_x, &full_bar[stage], 0, 0, step * KB);
+                        tma_load_3d(to, &tm_w, &full_bar[stage], 0, w_row, step * KB);
+                        tma_load_3d(to + w_bytes, &tm_x, &full_bar[stage], 0, x_row, step * KB);
                     } else {
 #pragma unroll 1
                         for (int b = 0; b < KB; ++b) {
-                            tma_load_3d(to + b * w_block, &tm_w, &full_bar[stage], (step * KB + b) * BLOCK_K, grp * a.rows, 0);
-                            tma_load_3d(to + w_bytes + b * TOKENS * BLOCK_K, &tm_x, &full_bar[stage], (step * KB + b) * BLOCK_K, 0, 0);
+                            tma_load_3d(to + b * w_block, &tm_w, &full_bar[stage], (step * KB + b) * BLOCK_K, w_row, 0);
+                            tma_load_3d(to + w_bytes + b * TOKENS * BLOCK_K, &tm_x, &full_bar[stage], (step * KB + b) * BLOCK_K, x_row, 0);
                         }
                     }
                     ++issued;
@@ -184,6 +235,7 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
                         phase ^= 1u;
                     }
                 }
+            }
             if (*abort_flag) drain(full_bar, a.stages, issued);
         }
         __syncwarp();
@@ -196,11 +248,20 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
         const int r = threadIdx.x;  // the row of the group that this thread finishes
         int stage = 0;
         uint32_t phase = 0;
-        for (int grp = blockIdx.x; grp < a.groups; grp += gridDim.x) {
-            const int64_t n = (int64_t)grp * a.rows + r;
+        if constexpr (GROUPED) {  // rows behind the last group are zeros
+            const int esz = p.out_dtype == FG_DTYPE_F32 ? 4 : 2;
+            for (int64_t row = min(max(a.offs[a.n_experts - 1], 0), (int)p.M) + (int64_t)blockIdx.x; row < p.M; row += gridDim.x) {
+                uint16_t* to = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p.c) + row * p.ld_c * esz);
+                for (int64_t i = threadIdx.x; i < p.N * (esz / 2); i += 32 * WARPS) to[i] = 0;
+            }
+        }
+        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+            const int ex = GROUPED ? item / a.groups : 0, expert = GROUPED ? ex_id[ex] : 0, m0 = GROUPED ? ex_first[ex] : 0;
+            const int tokens = GROUPED ? ex_count[ex] : (int)p.M;
+            const int64_t n = (int64_t)(GROUPED ? item % a.groups : item) * a.rows + r;
             const bool mine = r < a.rows && n < p.N;
-            const float sb = mine ? p.sb[p.sb_mode == FG_SCALE_VECTOR ? n : 0] : 0.0f;
-            const float bias = mine && p.bias ? load_bias(p.bias, p.bias_dtype, n) : 0.0f;
+            const float sb = mine ? p.sb[p.sb_mode == FG_SCALE_VECTOR ? expert * p.N + n : 0] : 0.0f;
+            const float bias = mine && p.bias ? load_bias(p.bias, p.bias_dtype, expert * a.bias_stride + n) : 0.0f;
             int acc[SPW][NT][4];
 #pragma unroll
             for (int s = 0; s < SPW; ++s)
@@ -253,22 +314,23 @@ __global__ void __launch_bounds__(THREADS, 1) int8_skinny_kernel(const __grid_co
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int m = 8 * j + 2 * t + (i & 1);
-                        if (m < p.M) atomicAdd(&sums[m * a.rows + 16 * strip + 8 * (i >> 1) + g], acc[s][j][i]);
+                        if (m < tokens) atomicAdd(&sums[m * a.rows + 16 * strip + 8 * (i >> 1) + g], acc[s][j][i]);
                     }
             }
             if (any_failed<32 * WARPS>(!ok)) break;
-            if (mine) {
-                for (int m = 0; m < p.M; ++m) {
-                    float v = sb * (sa_s[m] * (float)sums[m * a.rows + r]);
-                    sums[m * a.rows + r] = 0;
+            if (r < a.rows) {
+                for (int m = 0; m < tokens; ++m) {
+                    float v = sb * (sa_s[m0 + m] * (float)sums[m * a.rows + r]);
+                    sums[m * a.rows + r] = 0;  // also where the group reaches beyond the weight
+                    if (!mine) continue;
                     if (p.bias) v = (p.bias_after_round ? rounded(v, p.out_dtype) : v) + bias;
-                    const int64_t at = m * p.ld_c + n;
+                    const int64_t at = (int64_t)(m0 + m) * p.ld_c + n;
                     if (p.out_dtype == FG_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(p.c)[at] = __float2bfloat16_rn(v);
                     else if (p.out_dtype == FG_DTYPE_F16) reinterpret_cast<__half*>(p.c)[at] = __float2half_rn(v);
                     else reinterpret_cast<float*>(p.c)[at] = v;
                 }
             }
-            if (grp + gridDim.x < a.groups) any_failed<32 * WARPS>(false);  // the sums are zeros again
+            if (item + (int)gridDim.x < items) any_failed<32 * WARPS>(false);  // the sums are zeros again
         }
     }
     __syncthreads();
@@ -442,13 +504,14 @@ __global__ void __launch_bounds__(256, 1) int8_stream_kernel(const __grid_consta
 int byte_maps(StreamArgs& a, int kb, int token_rows, CUtensorMap* tm_w, CUtensorMap* tm_x) {
     const FgSkinny& p = a.p;
     a.wide = p.K % BLOCK_K == 0;
+    const uint64_t w_rows = (uint64_t)p.N * (uint64_t)(a.offs ? a.n_experts : 1);
     int rc;
     if (a.wide) {  // blocks of 128 bytes as the last dimension
         const uint64_t blocks = (uint64_t)(p.K / BLOCK_K);
-        rc = fg_byte_map(tm_w, p.b, BLOCK_K, (uint64_t)p.N, blocks, (uint64_t)p.ld_b, BLOCK_K, (uint32_t)a.rows, 3, (uint32_t)kb);
+        rc = fg_byte_map(tm_w, p.b, BLOCK_K, w_rows, blocks, (uint64_t)p.ld_b, BLOCK_K, (uint32_t)a.rows, 3, (uint32_t)kb);
         if (rc == FG_OK) rc = fg_byte_map(tm_x, p.a, BLOCK_K, (uint64_t)p.M, blocks, (uint64_t)p.ld_a, BLOCK_K, (uint32_t)token_rows, 3, (uint32_t)kb);
     } else {
-        rc = fg_byte_map(tm_w, p.b, (uint64_t)p.K, (uint64_t)p.N, 1, (uint64_t)p.ld_b, (uint64_t)p.ld_b * p.N, (uint32_t)a.rows, 3);
+        rc = fg_byte_map(tm_w, p.b, (uint64_t)p.K, w_rows, 1, (uint64_t)p.ld_b, (uint64_t)p.ld_b * w_rows, (uint32_t)a.rows, 3);
         if (rc == FG_OK) rc = fg_byte_map(tm_x, p.a, (uint64_t)p.K, (uint64_t)p.M, 1, (uint64_t)p.ld_a, (uint64_t)p.ld_a * p.M, (uint32_t)token_rows, 3);
     }
     return rc;
@@ -484,10 +547,10 @@ int launch_stream(StreamArgs& a, cudaStream_t st) {
     return FG_OK;
 }
 
-template <int NT, int SPW, int KB>
+template <int NT, int SPW, int KB, bool GROUPED>
 int launch(StreamArgs& a, cudaStream_t st) {
     const FgSkinny& p = a.p;
-    auto kernel = int8_skinny_kernel<NT, SPW, KB>;
+    auto kernel = int8_skinny_kernel<NT, SPW, KB, GROUPED>;
     static bool attr_done[64];
     static std::mutex mu;
     {
@@ -498,9 +561,10 @@ int launch(StreamArgs& a, cudaStream_t st) {
             done = true;
         }
     }
-    const int grid = a.groups < fg_num_sms() ? a.groups : fg_num_sms();
+    const int64_t items = (int64_t)a.groups * (GROUPED ? (p.M < a.n_experts ? p.M : a.n_experts) : 1);  // at most
+    const int grid = items < fg_num_sms() ? (int)items : fg_num_sms();
     const int64_t stage = (int64_t)KB * (a.rows + 8 * NT) * BLOCK_K;
-    const int64_t all = fg_cdiv(p.K, KB * BLOCK_K) * fg_cdiv(a.groups, grid);
+    const int64_t all = fg_cdiv(p.K, KB * BLOCK_K) * fg_cdiv(items, grid);
     const int64_t sums = (int64_t)8 * NT * a.rows * sizeof(int) + 1024;
     int64_t stages = (SMEM_BYTES - sums) / stage;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
@@ -516,22 +580,25 @@ int launch(StreamArgs& a, cudaStream_t st) {
 }
 
 // Stages of 20 to 48 KB: the lower a group, the more blocks of K.
+template <bool GROUPED>
 int launch_registers(StreamArgs& a, cudaStream_t st) {
     auto by_rows = [&](auto nt) -> int {
         constexpr int NT = decltype(nt)::value;
-        if (a.rows <= 16) return launch<NT, 1, 8>(a, st);
-        if (a.rows <= 32) return launch<NT, 2, 8>(a, st);
+        if (a.rows <= 16) return launch<NT, 1, 8, GROUPED>(a, st);
+        if (a.rows <= 32) return launch<NT, 2, 8, GROUPED>(a, st);
         if constexpr (NT <= 2) {
-            if (a.rows <= 64) return launch<NT, 2, 4>(a, st);
-            if (a.rows <= 128) return launch<NT, 2, 2>(a, st);
-            return launch<NT, 2, 1>(a, st);
+            if (a.rows <= 64) return launch<NT, 2, 4, GROUPED>(a, st);
+            if (a.rows <= 128) return launch<NT, 2, 2, GROUPED>(a, st);
+            return launch<NT, 2, 1, GROUPED>(a, st);
         }
         fg_set_error("groups of %d rows are built for up to 16 tokens", a.rows);
         return FG_ERR_UNSUPPORTED;
     };
-    const int64_t m = a.p.M;
-    return m <= 8 ? by_rows(std::integral_constant<int, 1>()) : m <= 16 ? by_rows(std::integral_constant<int, 2>())
-                                                                        : by_rows(std::integral_constant<int, 4>());
+    if (a.p.M <= 8) return by_rows(std::integral_constant<int, 1>());
+    if (a.p.M <= 16) return by_rows(std::integral_constant<int, 2>());
+    if constexpr (!GROUPED) return by_rows(std::integral_constant<int, 4>());
+    fg_set_error("at most 16 rows");
+    return FG_ERR_UNSUPPORTED;
 }
 
 int launch_tensor_memory(StreamArgs& a, cudaStream_t st) {
@@ -562,5 +629,36 @@ int fg_int8_skinny(const FgSkinny& p, cudaStream_t st) {
     // Measured, registers / TMEM: 2112 x 7168 5.6 / 10.7 us with 16 tokens, 7.2 / 10.6 with 32; 6144 x 4096 7.6 / 8.9 with 16,
     // 9.5 / 8.9 with 32; 24576 x 7168 33.3 / 33.1 and 39.1 / 33.2; 4096 x 14336 15.7 / 20.2 with 32, 21.8 / 19.7 with 33.
     const bool registers = p.M <= 16 || (p.M <= 32 && a.rows <= 32);
-    return registers ? launch_registers(a, st) : launch_tensor_memory(a, st);
+    return registers ? launch_registers<false>(a, st) : launch_tensor_memory(a, st);
+}
+
+// The same for experts: rows [offs[e - 1], offs[e]) of up to 16 in all times weight e.  One launch without tables of tiles, and groups
+// of weight rows that fit the SMs whatever the number of experts.  Measured against two launches and 128-row tiles: 1 row x 4096 x
+// 14336 11.4 us (43.2), 8 rows in 256 experts x 4096 x 7168 40.8 (45.7; the weights alone 35.9), x 7168 x 2048 23.9 (30.4), 16 rows in 8
+// experts x 28672 x 4096 131.6 (136.0).  From 17 rows on the tiles are as fast (84 us both, 90 % of the weights' stream).
+int fg_int8_skinny_grouped(const FgSkinny& p, const int32_t* offs, int n_experts, int64_t bias_stride, cudaStream_t st) {
+    FG_REQUIRE(fg_int8_is_skinny_grouped(p.M, p.N, n_experts) && p.M > 0 && p.N > 0 && p.K > 0 && p.K % 16 == 0, FG_ERR_UNSUPPORTED, "bad sizes");
+    StreamArgs a{};
+    a.p = p;
+    a.offs = offs;
+    a.n_experts = n_experts;
+    a.bias_stride = bias_stride;
+    a.status = fg_status_word_device_ptr();
+    // The height whose groups, over as many experts as can have rows, take the least time on an SM: their weight rows, the tokens'
+    // rows beside them, and an epilogue that is worth 64 KB of the weight.
+    const int64_t experts = p.M < n_experts ? p.M : n_experts;
+    int64_t least = INT64_MAX;
+    for (int rows = MAX_ROWS; rows >= 16; rows -= 16) {
+        const int64_t most = fg_cdiv(fg_cdiv(p.N, rows) * experts, fg_num_sms()) * (rows + (p.M <= 8 ? 8 : 16) + 65536 / p.K);
+        if (most < least) {
+            least = most;
+            a.rows = rows;
+        }
+    }
+    a.groups = (int)fg_cdiv(p.N, a.rows);
+    return launch_registers<true>(a, st);
+}
+
+bool fg_int8_is_skinny_grouped(int64_t M, int64_t N, int n_experts) {
+    return M <= 16 && n_experts <= 1024 && N * n_experts < (1ll << 31) - MAX_ROWS;
 }

@@ -272,6 +272,13 @@ int scaled_grouped_mm(int operand, void* c, const void* a, const void* b, const 
     const Workspace ws = carve_grouped_mm(workspace, m_total, num_groups, tile);
     FG_REQUIRE(workspace_bytes >= ws.bytes, FG_ERR_INVALID_ARGUMENT, "workspace holds %lld bytes, needs %lld",
                (long long)workspace_bytes, (long long)ws.bytes);
+    FG_REQUIRE(out_dtype == FG_DTYPE_BF16 || out_dtype == FG_DTYPE_F16 || out_dtype == FG_DTYPE_F32, FG_ERR_INVALID_ARGUMENT,
+               "bad out_dtype %d", out_dtype);
+    FG_REQUIRE(ld_a >= K, FG_ERR_INVALID_ARGUMENT, "row stride smaller than K");
+    if (operand == 1 && fg_int8_is_skinny_grouped(m_total, N, num_groups))
+        return fg_int8_skinny_grouped(FgSkinny{c, (const int8_t*)a, (const int8_t*)b, scale_a, scale_b, bias, m_total, N, K, ld_a, K, ld_c,
+                                               FG_SCALE_VECTOR, FG_SCALE_VECTOR, out_dtype, FG_DTYPE_F32, 0},
+                                      offs, num_groups, bias_stride_g, st);
     // int8: the rows past the last group become zeros
     const FgTail tail{operand == 1 ? c : nullptr, ld_c, N, out_dtype == FG_DTYPE_F32 ? 4 : 2};
     int rc = fg_group_tiles(offs, num_groups, m_total, tile, ws.sorted_ids, ws.max_pad, ws.expert_ids, ws.n_blocks,

@@ -249,6 +249,44 @@ def test_grouped(sizes, n, k):
     _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs), _grouped_definition(a, b, a_s, b_s, offs))
 
 
+FEW = [[1], [16], [0, 1, 0], [8, 8], [0, 15, 0, 0], [3, 0, 2, 1, 0, 0, 4], [1] * 16, [0] * 300 + [2] + [0] * 10 + [7], [0] * 1022 + [5, 1],
+       [2] + [0] * 1023, [0, 9, 0, 7], [0, 0, 0]]
+
+
+@pytest.mark.parametrize("sizes", FEW, ids=[f"{len(s)}x{sum(s)}" for s in FEW])
+@pytest.mark.parametrize("n,k", [(16, 16), (515, 272), (4096, 128), (3000, 1040)])
+@pytest.mark.parametrize("tail", [0, 2])
+def test_grouped_few_rows(sizes, n, k, tail):
+    if len(sizes) > 500 and n * k > 200000:
+        n, k = 264, 384
+    a, b, a_s, b_s, offs, g = _grouped(sizes, n, k, tail=tail)
+    if a.shape[0] == 0:
+        return
+    junk = [torch.full((a.shape[0], n), float("nan"), device="cuda") for _ in range(4)]  # memory that is reused
+    del junk
+    want = _grouped_definition(a, b, a_s, b_s, offs)
+    for out in (torch.bfloat16, torch.float32):
+        _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs, output_dtype=out), want)
+    group = torch.repeat_interleave(torch.arange(len(sizes), device="cuda"), torch.tensor(sizes, device="cuda"))
+    for bias in (torch.randn(n, device="cuda", generator=g), torch.randn(len(sizes), n, device="cuda", generator=g)):
+        got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs, bias, torch.float16)
+        real = a.shape[0] - tail
+        _check(got[:real], want[:real], bias.expand(len(sizes), n)[group])
+        assert not got[real:].any()
+    assert _cabi.device_status() == 0
+
+
+def test_grouped_ends_that_the_kernel_before_writes():
+    a, b, a_s, b_s, offs, g = _grouped([4] * 4, 4096, 1024)
+    kept = []
+    for i in range(12):
+        ids = torch.randint(0, 4, (16, 1), device="cuda", generator=g)
+        rows, row_s, plan = flag_gems.moe_permute(a, ids, 4, scale=a_s)
+        kept.append((rows, row_s, plan.offs, flag_gems.w8a8_int8_grouped_mm(rows, b, row_s, b_s, plan.offs)))
+    for rows, row_s, ends, c in kept:
+        _check(c, _grouped_definition(rows, b, row_s, b_s, ends))
+
+
 @pytest.mark.parametrize("sizes", [[700, 0, 130, 400], [100, 250, 97, 3, 300], [1300, 700, 900], [2100, 1500]], ids=str)
 @pytest.mark.parametrize("n", [2112, 4096, 6200])
 def test_grouped_tiles_of_every_width(sizes, n):
