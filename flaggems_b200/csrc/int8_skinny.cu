@@ -140,7 +140,7 @@ __device__ int experts_with_rows(const int32_t* offs, int n_experts, int rows, i
         const int e = (warp * EACH + i) * 32 + lane;
         const bool in = warp < WARPS && e < n_experts;
         lo[i] = in && e > 0 ? min(max(offs[e - 1], 0), rows) : 0;
-        n[i] = in ? min(offs[e], rows) - lo[i] : 0;
+        n[i] = in ? min(max(offs[e], 0), rows) - lo[i] : 0;
     }
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {

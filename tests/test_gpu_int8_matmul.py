@@ -276,6 +276,19 @@ def test_grouped_few_rows(sizes, n, k, tail):
     assert _cabi.device_status() == 0
 
 
+def test_grouped_few_rows_of_ends_out_of_range():
+    a, b, a_s, b_s, offs, _ = _grouped([2, 0, 3, 1], 515, 272, tail=3)
+    want = _grouped_definition(a, b, a_s, b_s, offs)
+    low, high = torch.iinfo(torch.int32).min, torch.iinfo(torch.int32).max
+    ends = torch.tensor([2, low, 5, 6], dtype=torch.int32, device="cuda")  # groups 0 and 2 share the first two rows
+    got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, ends, output_dtype=torch.float32)
+    _check(got[2:], want[2:])
+    ends = torch.tensor([2, 2, 5, high], dtype=torch.int32, device="cuda")  # the last group takes what is left
+    want[5:] = _definition(a[5:], b[3], a_s[5:], b_s[3])
+    _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, ends, output_dtype=torch.float32), want)
+    assert _cabi.device_status() == 0
+
+
 def test_grouped_ends_that_the_kernel_before_writes():
     a, b, a_s, b_s, offs, g = _grouped([4] * 4, 4096, 1024)
     kept = []
