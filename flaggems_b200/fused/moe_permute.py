@@ -134,7 +134,8 @@ def moe_permute(
     zeros (their scales ones) and get no gradient back.
 
     Returns ``(rows [tokens * topk, hidden], row_scale or None, plan)``; ``plan.offs`` is what
-    ``w8a8_int8_grouped_mm`` and ``scaled_grouped_mm`` take.  Differentiable in ``hidden_states``, once.
+    ``w8a8_int8_grouped_mm`` and ``scaled_grouped_mm`` take.  Differentiable in ``hidden_states``, once.  A step that is
+    captured into a CUDA graph with its backward pass takes leaves of its own, as with every operator of torch.
     """
     logger.debug("GEMS MOE PERMUTE")
     if hidden_states.is_cuda:
@@ -156,11 +157,16 @@ def moe_permute(
         assert scale.shape[0] == x.shape[0], f"{x.shape[0]} tokens, {scale.shape[0]} rows of scales"
         if scale.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("scale has no gradient")
+    if expert_map is not None:
+        assert expert_map.dim() == 1 and expert_map.numel() > 0, "expert_map must be 1-D and not empty"
+        if expert_map.dtype not in (torch.int32, torch.int64):
+            raise NotImplementedError(f"expert_map must be int32 or int64, got {expert_map.dtype}")
     _check_devices(x, topk_ids, scale, expert_map)
     topk_ids = topk_ids.contiguous()
     if expert_map is not None:
-        assert expert_map.dim() == 1 and expert_map.numel() > 0, "expert_map must be 1-D and not empty"
-        expert_map = expert_map.to(torch.int32).contiguous()
+        if expert_map.dtype == torch.int64:  # what is outside the range stays outside in 32 bits
+            expert_map = expert_map.clamp(-1, num_experts).to(torch.int32)
+        expert_map = expert_map.contiguous()
     call = _Permute.apply if torch.is_grad_enabled() and x.requires_grad else _permute
     rows, row_scale, *plan = call(x, topk_ids, num_experts, scale, expert_map)
     return rows, row_scale, MoEPermutation(*plan)

@@ -438,3 +438,36 @@ def test_an_int8_expert_layer_of_its_parts():
     want = (q.double() @ w1[0].double().t()) * q_s.double() * s1[0].double()
     assert bool(((up.double() - want).abs() <= want.abs() * (2.0 ** -8 + 4 * F32)).all())
     assert _cabi.device_status() == 0
+
+
+@pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("t", [9, 3000])
+def test_ids_and_maps_beyond_32_bits(ids_dtype, t):
+    g = _gen(t)
+    e, k, h = 6, 4, 40
+    x = torch.randn(t, h, device="cuda", generator=g)
+    ids = torch.randint(0, 12, (t, k), device="cuda", generator=g).to(ids_dtype)
+    if ids_dtype == torch.int64:
+        ids[::3, 0] += 2 ** 32  # no id of the map
+        ids[1::3, 1] -= 2 ** 33
+    else:
+        ids[::3, 0] = torch.iinfo(torch.int32).max
+        ids[1::3, 1] = torch.iinfo(torch.int32).min
+    expert_map = torch.tensor([5, 0, 2 ** 32, -1, 2 ** 32 + 3, 1, 2, -2 ** 32, 3, 4, 2 ** 40 - 1, 6], device="cuda")
+    rows, _, plan = flag_gems.moe_permute(x, ids, e, expert_map=expert_map)
+    _same_plan(plan, _plan(ids, e, expert_map))
+    _check_permuted(x, rows, plan, k)
+
+
+def test_inference_mode():
+    g = _gen(5)
+    x, w = torch.randn(20, 64, device="cuda", generator=g).bfloat16(), torch.rand(20, 2, device="cuda", generator=g)
+    ids = _ids(20, 8, 2, g)
+    rows, _, plan = flag_gems.moe_permute(x, ids, 8)
+    want = flag_gems.moe_unpermute(rows, plan, w)
+    with torch.inference_mode():
+        rows2, _, plan2 = flag_gems.moe_permute(x, ids, 8)
+        assert torch.equal(flag_gems.moe_unpermute(rows2, plan2, w), want)
+        plan2.row_of_slot.add_(0)  # an ordinary tensor in there
+        assert rows2.is_inference() and plan2.row_of_slot.is_inference() and plan2.offs.is_inference()
+    _same_plan([t.clone() for t in plan2], plan)

@@ -150,3 +150,13 @@ def test_entry_points_check_their_sizes():
     refused(lib.fg_moe_unpermute_backward(p, p, p, p, p, p, 5, 4, 2, 8, 8, 8, 8, 2, 0, None), -1, "bad weight dtype")
     refused(lib.fg_moe_unpermute_backward(p, p, p, None, p, p, 2, 4, 2, 8, 8, 8, 8, 2, 0, None), -1, "null pointer")
     assert lib.fg_moe_unpermute_backward(p, p, p, p, p, p, 2, 0, 2, 8, 8, 8, 8, 2, 0, None) == 0
+
+
+@pytest.mark.parametrize("expert_map,error,text", [
+    (torch.zeros(4), NotImplementedError, "expert_map must be int32 or int64"),
+    (torch.zeros(0, dtype=torch.int32), AssertionError, "1-D and not empty"),
+    (torch.zeros(2, 2, dtype=torch.int32), AssertionError, "1-D and not empty"),
+])
+def test_expert_maps(expert_map, error, text):
+    with pytest.raises(error, match=text):
+        _permute(expert_map=expert_map)
