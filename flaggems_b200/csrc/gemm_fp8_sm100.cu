@@ -32,6 +32,7 @@
 
 #include "common.cuh"
 #include "ptx_sm100.cuh"
+#include "store_rows.cuh"
 
 using namespace fgptx;
 namespace cg = cooperative_groups;
@@ -69,6 +70,7 @@ struct GemmParams {
     int bias_dtype;  // element type of bias (the output type, or fp32 when the output is e4m3 / for grouped mm)
     int64_t bias_stride_e;  // grouped: elements between the bias rows of consecutive experts (0: one row)
     int c_vec_ok;  // rows of C are 16-byte aligned
+    int c_align;   // int8: what the rows of C begin at multiples of (fg_row_align)
     const float* sa;
     const float* sb;
     const void* bias;
@@ -298,14 +300,16 @@ __device__ __forceinline__ TileCoord tile_coord(int t, int num_m, int num_n) {
 // applies the per-row x per-column scales); 2 / 3 = bf16 / f16 (kind::f16) for the unquantised and
 // weight-only-quantised expert GEMMs.  The main loop is written in bytes (a K block is 128 bytes of a
 // K-major row, an MMA consumes 32 of them), so a 16-bit product of K elements runs as 2K bytes.
+// BY_ROWS: results go out by fg_store_rows where a warp's rows are evenly spaced.
 template <int BN, bool BLOCK_SCALED, bool FUSE_SILU, bool SMALL_A, bool SPLITK, bool PAIR = false, bool ASTORE = false,
-          int OPK = 0>
+          int OPK = 0, bool BY_ROWS = false>
 __global__ void __launch_bounds__(Cfg<BN, SMALL_A, PAIR, ASTORE>::THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                 const GemmParams p) {
     using C = Cfg<BN, SMALL_A, PAIR, ASTORE, !BLOCK_SCALED && !SPLITK>;
     static_assert(!ASTORE || (BLOCK_SCALED && !SPLITK), "the store warp serves the block-scaled tiles");
     constexpr bool INT8 = OPK == 1;
+    static_assert(!BY_ROWS || (INT8 && !FUSE_SILU), "built for int8 products");
     // int8 products of up to 128 rows are int8_skinny.cu's; 16-bit operands serve the grouped tiles
     static_assert(OPK == 0 || (!BLOCK_SCALED && !SPLITK && !SMALL_A), "these are built for e4m3 operands");
     // accumulator word -> fp32
@@ -805,6 +809,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                 // cost a global-memory latency per column of a tile (40 us of the 58 us of a single-wave
                 // product such as 16 x 28672 x 4096).
                 const float sa = p.sa_mode == FG_SCALE_VECTOR ? p.sa[srow] : p.sa[0];
+                FgRows rows{};
+                if constexpr (BY_ROWS) rows = fg_rows(out_ptr, row_ok, lane, p.ld_c * esz);
                 float* col_scale = reinterpret_cast<float*>(epi_stage_base + C::EPI_WARPS * C::EPI_STAGE_BYTES + ew * C::COL_BYTES);
                 float* col_bias = col_scale + C::COLS;
                 if constexpr (!SPLITK) {
@@ -881,10 +887,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     }
                     if constexpr (!SPLITK) {
                         const int nc = min(32, p.n_out - col);
-                        if (nc == 32 && p.c_vec_ok && esz == 2)
+                        if (BY_ROWS && rows.even) {
+                            if (nc > 0) fg_store_rows(epi_stage, lane, v, rows, p.ld_c * esz, (int64_t)col * esz, nc, p.out_dtype, p.c_align);
+                        } else if (nc == 32 && p.c_vec_ok && esz == 2) {
                             store_chunk_coalesced(epi_stage, lane, v, out_ptr, row_ok, col, p.out_dtype);
-                        else if (row_ok && nc > 0)
+                        } else if (row_ok && nc > 0) {
                             store_chunk(out_ptr, col, v, nc, p.out_dtype, p.c_vec_ok);
+                        }
                     }
                 }
                 tc_fence_before_sync();
@@ -1293,10 +1302,10 @@ bool short_run(int64_t tiles) { return tiles <= 2 * (int64_t)fg_num_sms(); }
 // No block scales: with block scales the accumulator of every K block has to make the round
 // trip MMA -> both CTAs' epilogues -> MMA through cluster-wide barriers, and that latency costs
 // more than the halved B traffic saves (measured: about half the single-CTA throughput).
-template <bool SILU, int OPK>
+template <bool SILU, int OPK, bool BY_ROWS = false>
 int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, int pair_tiles, cudaStream_t st) {
     using C = Cfg<256, false, true, false, true>;
-    auto kernel = gemm_fp8_kernel<256, false, SILU, false, false, true, false, OPK>;
+    auto kernel = gemm_fp8_kernel<256, false, SILU, false, false, true, false, OPK, BY_ROWS>;
     static int max_clusters_dev[64];
     static std::mutex mu;
     std::lock_guard<std::mutex> lock(mu);
@@ -1337,10 +1346,10 @@ bool pair_enabled() {
     return v != 0;
 }
 
-template <int BN, bool BS, bool SILU, bool SMALL_A = false, bool ASTORE = false, int OPK = 0>
+template <int BN, bool BS, bool SILU, bool SMALL_A = false, bool ASTORE = false, int OPK = 0, bool BY_ROWS = false>
 int launch_inst(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, int max_tiles, cudaStream_t st) {
     using C = Cfg<BN, SMALL_A, false, ASTORE, !BS>;
-    auto kernel = gemm_fp8_kernel<BN, BS, SILU, SMALL_A, false, false, ASTORE, OPK>;
+    auto kernel = gemm_fp8_kernel<BN, BS, SILU, SMALL_A, false, false, ASTORE, OPK, BY_ROWS>;
     static bool attr_done[64];
     static std::mutex mu;
     {
@@ -1374,6 +1383,7 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     p.status = fg_status_word_device_ptr();
     const int esz = out_elem_size(p.out_dtype);
     p.c_vec_ok = ((uintptr_t)p.c % 16 == 0) && ((p.ld_c * esz) % 16 == 0);
+    p.c_align = fg_row_align(p.c, p.ld_c * esz);
 
     const int64_t m_tiles = p.grouped ? p.M / p.block_rows : fg_cdiv(p.M, BLOCK_M);
     const int sms = fg_num_sms();
@@ -1449,13 +1459,21 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     rc = fg_byte_map(&tb, b, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)num_experts, (uint64_t)ld_b,
                   (uint64_t)ld_b * (uint64_t)p.N, (uint32_t)(fuse_silu ? bn / 2 : pair ? p.tile_n / 2 : p.tile_n), 3);
     if (rc != FG_OK) return rc;
+    // int8 results of 32 bits, or in rows that are not aligned, are written row by row (store_rows.cuh), and so are those of more than
+    // one wave of tiles, where that takes fewer instructions from the next tile's: 2048 x 7168 x 2048 29.4 us (30.9), 3859 x 6144 x
+    // 4096 70.4 (73.4).  A single wave waits for the larger code at its end: 129 x 7168 x 2048 11.1 us, without 10.7.
+    const bool by_rows = p.int8 == 1 && !fuse_silu && (esz == 4 || !p.c_vec_ok || (!p.grouped && tiles > sms));
     if (pair) {
         FG_REQUIRE(pair_tiles < (1ll << 30), FG_ERR_UNSUPPORTED, "too many tiles");
         auto by_kind = [&](auto silu_tag) -> int {
             constexpr bool S = decltype(silu_tag)::value;
             switch (p.int8) {
                 case 0: return launch_pair<S, 0>(ta, tb, p, (int)pair_tiles, st);
-                case 1: return launch_pair<S, 1>(ta, tb, p, (int)pair_tiles, st);
+                case 1:
+                    if constexpr (!S) {
+                        if (by_rows) return launch_pair<S, 1, true>(ta, tb, p, (int)pair_tiles, st);
+                    }
+                    return launch_pair<S, 1>(ta, tb, p, (int)pair_tiles, st);
                 case 2: return launch_pair<S, 2>(ta, tb, p, (int)pair_tiles, st);
                 default: return launch_pair<S, 3>(ta, tb, p, (int)pair_tiles, st);
             }
@@ -1467,12 +1485,17 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     if (p.int8) {
         FG_REQUIRE(!block_scaled && (p.int8 == 1 || p.grouped), FG_ERR_UNSUPPORTED,
                    "int8 operands take no block scales, and 16-bit operands are built for the grouped expert GEMMs");
-        if (bn == 64) return launch_inst<64, false, false, false, false, 1>(ta, tb, p, t, st);
+        if (bn == 64) return by_rows ? launch_inst<64, false, false, false, false, 1, true>(ta, tb, p, t, st)
+                                     : launch_inst<64, false, false, false, false, 1>(ta, tb, p, t, st);
         auto by_kind = [&](auto bn_tag, auto silu_tag) -> int {
             constexpr int B = decltype(bn_tag)::value;
             constexpr bool S = decltype(silu_tag)::value;
             switch (p.int8) {
-                case 1: return launch_inst<B, false, S, false, false, 1>(ta, tb, p, t, st);
+                case 1:
+                    if constexpr (!S) {
+                        if (by_rows) return launch_inst<B, false, S, false, false, 1, true>(ta, tb, p, t, st);
+                    }
+                    return launch_inst<B, false, S, false, false, 1>(ta, tb, p, t, st);
                 case 2: return launch_inst<B, false, S, false, false, 2>(ta, tb, p, t, st);
                 default: return launch_inst<B, false, S, false, false, 3>(ta, tb, p, t, st);
             }

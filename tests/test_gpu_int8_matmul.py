@@ -207,6 +207,19 @@ def test_cutlass_scaled_mm(m, n, k, bias, out):
     _check(c, _definition(a, b, a_s, b_s), t, rounded_before_bias=bias)
 
 
+@pytest.mark.parametrize("m,n", [(33, 700), (64, 31), (97, 9471), (128, 33), (131, 65), (300, 2845), (1037, 2050), (2500, 6145)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("off", [0, 1, 2, 8])
+def test_results_between_others(m, n, out, off):
+    """Rows that begin at any value, in a wider matrix whose other values stay as they are."""
+    a, b, a_s, b_s, _ = _operands(m, n, 272, seed=n)
+    wide = torch.full((m, (n + off + 31) // 16 * 16), 7.0, dtype=out, device="cuda")
+    flag_gems.cutlass_scaled_mm(wide[:, off:off + n], a, b.t(), a_s, b_s)
+    _check(wide[:, off:off + n], _definition(a, b, a_s, b_s))
+    assert bool((wide[:, :off] == 7).all()) and bool((wide[:, off + n:] == 7).all())
+    assert _cabi.device_status() == 0
+
+
 def test_cutlass_scaled_mm_refusals():
     a, b, a_s, b_s, _ = _operands(16, 128, 256)
     c = torch.empty(16, 128, dtype=torch.bfloat16, device="cuda")
@@ -311,6 +324,14 @@ def test_grouped_tiles_of_every_width(sizes, n):
     got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs, bias, torch.float16)
     _check(got[:-5], want[:-5], bias[group])
     assert not got[-5:].any()
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("sizes", [[700, 0, 130, 33], [1300, 1], [20] * 8], ids=str)
+@pytest.mark.parametrize("n", [31, 2050, 2845])
+def test_grouped_rows_of_any_alignment(out, sizes, n):
+    a, b, a_s, b_s, offs, _ = _grouped(sizes, n, 272, seed=n, tail=3)
+    _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs, output_dtype=out), _grouped_definition(a, b, a_s, b_s, offs))
 
 
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
