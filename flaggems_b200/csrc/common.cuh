@@ -158,11 +158,11 @@ __device__ __forceinline__ void fg_pdl_trigger() { asm volatile("griddepcontrol.
 // Launches `kernel` that way (or, without `early`, after everything before it), with clusters of `cluster` CTAs
 // when cluster > 1.
 template <typename... Params, typename... Args>
-cudaError_t fg_launch_when(bool early, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t st,
+cudaError_t fg_launch_when(bool early, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                            unsigned cluster, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(block, 1, 1);
+    cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -183,12 +183,12 @@ cudaError_t fg_launch_when(bool early, void (*kernel)(Params...), dim3 grid, uns
 }
 
 template <typename... Params, typename... Args>
-cudaError_t fg_launch(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, unsigned cluster,
+cudaError_t fg_launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, unsigned cluster,
                       Args&&... args) {
     // Not where the grid fills more than half of the chip's thread slots: its CTAs would sit in them, waiting, while
     // another stream (a layer's shared expert) has work for the SMs.  A layer of 8192 tokens takes 6018 us with every
     // kernel launched early, 5827 with this rule and that of the products, and took 5772 before there were early launches.
-    const bool early = (int64_t)grid.x * grid.y * block <= 1024 * (int64_t)fg_num_sms();
+    const bool early = (int64_t)grid.x * grid.y * block.x * block.y <= 1024 * (int64_t)fg_num_sms();
     return fg_launch_when(early, kernel, grid, block, smem, st, cluster, args...);
 }
 

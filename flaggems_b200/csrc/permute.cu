@@ -128,13 +128,21 @@ struct RowArgs {
     const float* scale;
     int64_t ld_scale;
     int topk;
-    int64_t n_rows;
+    int64_t tokens, n_rows;
     void* rows;
     int units;  // per row
     float* row_scale;
     int scale_cols;
 };
 constexpr int SLOTS_AT_ONCE = 8;
+
+// The token of a thread: the CTA's, or with SHARED one per threadIdx.y.  With one per CTA it is the same in all threads, what is found
+// by it too, and that takes fewer registers: 16381 x 2 fp16 rows of 4096 are summed in 70 us, in 89 with the general form.
+template <bool SHARED>
+__device__ __forceinline__ int64_t token_of_thread() {
+    if constexpr (SHARED) return (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    else return blockIdx.x;
+}
 
 struct __align__(32) Unit32 {
     uint4 lo, hi;
@@ -219,38 +227,42 @@ __global__ void __launch_bounds__(256) scan_chunks_kernel(SortArgs s, ChunkTable
     }
 }
 
-// Many slots, third launch, one CTA per token: its row is read once and written slot after slot.  Bound by the writes, which
+// Many slots, third launch, one CTA per token, or per several (threadIdx.y) of narrow rows: a row is read once and written slot after slot.  Bound by the writes, which
 // are topk times the reads, and by the rate of a copy.  Few registers (and so many CTAs, a row each, under way) matter more
 // than pieces per thread, and accesses of 32 bytes more than those of 16: 8192 x 8 rows of 14336 bytes take 164 us (6.4 TB/s
 // of the 6.6 of a copy), 178 with two pieces of 16 bytes per thread; rows of 7168 bytes 84, 88, and 98 with four pieces and the
 // slots' rows in registers, 91-97 as bulk copies through a ring in shared memory.
-// UNIT: the bytes of a load, 32 or 16 where everything is aligned to that.
-template <typename UNIT>
+// UNIT: the bytes of a load, the most that everything is aligned to.
+template <typename UNIT, bool SHARED>
 __global__ void __launch_bounds__(512) permute_rows_kernel(SortArgs s, ChunkTable ct, RowArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
-    constexpr int PIECES = sizeof(UNIT) == 32 ? 1 : 2, SLOTS = 32;
-    __shared__ int32_t row_s[SLOTS];
-    const int64_t t = blockIdx.x;
+    constexpr int PIECES = sizeof(UNIT) == 32 ? 1 : 2, SLOTS = 32, MAX_TOKENS = SHARED ? 32 : 1;
+    __shared__ int32_t row_s[MAX_TOKENS * SLOTS];
+    const int64_t t = token_of_thread<SHARED>(), t0 = SHARED ? t - threadIdx.y : t;
+    const int tokens = SHARED ? (int)blockDim.y : 1, units = !SHARED || t < a.tokens ? a.units : 0;
     UNIT piece[PIECES];
-    load_pieces(a, t, threadIdx.x, piece);
+    if (units) load_pieces(a, t, threadIdx.x, piece);
     for (int k0 = 0; k0 < a.topk; k0 += SLOTS) {
         const int slots = min(SLOTS, a.topk - k0);
-        if ((int)threadIdx.x < slots) {
-            const int64_t slot = t * a.topk + k0 + threadIdx.x;
+        for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < tokens * slots; i += tokens * blockDim.x) {
+            const int y = SHARED ? i / slots : 0, k = i - y * slots;
+            if (SHARED && t0 + y >= a.tokens) break;
+            const int64_t slot = (t0 + y) * a.topk + k0 + k;
             const int rank = s.row_of_slot[slot], e = expert_of(s, slot);
             const int32_t row = ct.table[(int64_t)e * ct.n_chunks + (int)slot / ct.chunk].x + rank;
             s.slot_of_row[row] = (int32_t)slot;
-            row_s[threadIdx.x] = s.row_of_slot[slot] = e < s.num_experts ? row : ~row;
+            row_s[y * SLOTS + k] = s.row_of_slot[slot] = e < s.num_experts ? row : ~row;
         }
         __syncthreads();
-        for (int v0 = threadIdx.x; v0 < a.units; v0 += PIECES * blockDim.x) {
+        const int32_t* my_rows = row_s + (SHARED ? threadIdx.y * SLOTS : 0);
+        for (int v0 = threadIdx.x; v0 < units; v0 += PIECES * blockDim.x) {
             if (v0 >= PIECES * (int)blockDim.x || k0 > 0) load_pieces(a, t, v0, piece);
 #pragma unroll 1
-            for (int k = 0; k < slots; ++k) store_pieces(a, row_s[k], v0, piece);
+            for (int k = 0; k < slots; ++k) store_pieces(a, my_rows[k], v0, piece);
         }
-        if (a.scale_cols)
-            for (int k = 0; k < slots; ++k) store_scales(a, t, k, row_s[k]);
+        if (a.scale_cols && (!SHARED || t < a.tokens))
+            for (int k = 0; k < slots; ++k) store_scales(a, t, k, my_rows[k]);
         __syncthreads();
     }
 }
@@ -366,7 +378,7 @@ struct SumArgs {
     int w_dtype;
     int64_t ld_w;
     int topk;
-    int64_t H;
+    int64_t tokens, H;
     void* out;  // [T, H]
     // backward
     const void* d_out;  // [T, H], row stride ld_d_out
@@ -412,15 +424,16 @@ __device__ __forceinline__ void load_slots(const SumArgs& a, int64_t t, int k0, 
         if (row[k] < 0 || row[k] >= a.n_rows) row[k] = -1;
 }
 
-// One CTA per token (and per part of its columns, blockIdx.y), sums in fp32 in slot order.  A thread has K slots
+// One CTA per token and per part of its columns (blockIdx.y), or per several tokens (threadIdx.y), sums in fp32 in slot order.  A thread has K slots
 // of U pieces in flight, eight loads whatever the number of slots.
-template <typename T, int V, int K>
+template <typename T, int V, int K, bool SHARED>
 __global__ void __launch_bounds__(256) unpermute_kernel(SumArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
     constexpr int U = K >= 8 ? 1 : 8 / K;
     using P = Piece<T, V>;
-    const int64_t t = blockIdx.x;
+    const int64_t t = token_of_thread<SHARED>();
+    if (SHARED && t >= a.tokens) return;
     const T* rows = reinterpret_cast<const T*>(a.rows);
     const int64_t step = (int64_t)blockDim.x * V;
     int32_t row[K];
@@ -461,24 +474,26 @@ __global__ void __launch_bounds__(256) unpermute_kernel(SumArgs a) {
     }
 }
 
-// One CTA per token: d_out[t] times the weight into the gradient of every row of the token, and its product with
+// One CTA per token, or per several (threadIdx.y, whole warps each): d_out[t] times the weight into the gradient of every row of the token, and its product with
 // the row into the gradient of the weight, slot after slot.  d_out is read once where a row is up to four pieces per
 // thread (16 KB), everything else is read and written once; the products are summed in a fixed order: a thread's columns, the
 // lanes, the warps.  Bound by HBM: 8192 x 8 bf16 rows of 7168 (2.0 GB) take 307 us, 6.5 TB/s, which is the rate of a
 // copy.  More slots in flight per thread cost registers and with them CTAs (404 us with two slots at once); streaming
 // loads and stores (.cs) take 315.
-template <typename T, int V>
+template <typename T, int V, bool SHARED>
 __global__ void __launch_bounds__(256, 4) unpermute_backward_kernel(SumArgs a) {
     fg_pdl_wait();
     fg_pdl_trigger();
     constexpr int U = 4, K = 32;  // pieces per thread and round, slots whose sums are parked at once
     using P = Piece<T, V>;
     __shared__ float part[8][K];
-    const int64_t t = blockIdx.x;
+    const int64_t t = token_of_thread<SHARED>();
+    const bool live = !SHARED || t < a.tokens;
     const T* rows = reinterpret_cast<const T*>(a.rows);
     const T* d_out = reinterpret_cast<const T*>(a.d_out) + t * a.ld_d_out;
     T* d_rows = reinterpret_cast<T*>(a.d_rows);
-    const int step = (int)blockDim.x * V, first = (int)threadIdx.x * V, H = (int)a.H;
+    const int step = (int)blockDim.x * V, first = (int)threadIdx.x * V, H = live ? (int)a.H : 0;
+    const int first_warp = SHARED ? (int)(threadIdx.y * blockDim.x) >> 5 : 0;
     const bool one_round = H <= U * step;
     typename P::Raw g[U];
     auto load_g = [&](int c) {
@@ -491,7 +506,7 @@ __global__ void __launch_bounds__(256, 4) unpermute_backward_kernel(SumArgs a) {
         const int slots = min(K, a.topk - k0);
 #pragma unroll 1
         for (int k = 0; k < slots; ++k) {
-            const int32_t r = a.row_of_slot[t * a.topk + k0 + k];
+            const int32_t r = live ? a.row_of_slot[t * a.topk + k0 + k] : -1;
             const int64_t row = r < 0 ? ~r : r;
             const bool real = r >= 0 && row < a.n_rows;
             const float w = real && a.weights ? load_weight(a.weights, a.w_dtype, t * a.ld_w + k0 + k) : 1.0f;
@@ -526,14 +541,14 @@ __global__ void __launch_bounds__(256, 4) unpermute_backward_kernel(SumArgs a) {
             if (a.d_w) {
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-                if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5][k] = dot;
+                if ((threadIdx.x & 31) == 0) part[first_warp + (threadIdx.x >> 5)][k] = dot;
             }
         }
         if (a.d_w) {
             __syncthreads();
-            if ((int)threadIdx.x < slots) {
+            if ((int)threadIdx.x < slots && live) {
                 float sum = 0.0f;
-                for (int i = 0; i < (int)blockDim.x / 32; ++i) sum += part[i][threadIdx.x];
+                for (int i = 0; i < (int)blockDim.x / 32; ++i) sum += part[first_warp + i][threadIdx.x];
                 store_weight(a.d_w, a.w_dtype, t * a.topk + k0 + threadIdx.x, sum);
             }
             __syncthreads();
@@ -555,6 +570,19 @@ int by_type(int dtype, F&& f) {
 
 // Threads of a CTA that walks a row of n pieces: few iterations, no more threads than pieces (in whole warps).
 unsigned threads_for(int64_t n) { return n >= 256 ? 256u : (unsigned)(n < 32 ? 32 : (n + 31) / 32 * 32); }
+
+// Several tokens share a CTA of 256 threads where one is served by fewer and moves few bytes, while four CTAs per SM are left: the
+// chip starts a CTA per 1.1 ns, in which 7 KB are moved.  Measured, a CTA per token / shared: 16384 x 8 rows of 128 bytes permuted in
+// 24.0 / 11.5 us and summed in 19.0 / 4.8, 16384 x 2 rows of 1024 bytes 22.9 / 13.7 and 18.8 / 12.8.
+dim3 block_of_tokens(unsigned threads, int64_t T, int64_t bytes_per_token) {
+    unsigned tokens = 1;
+    if (bytes_per_token <= 16384)
+        while (2 * tokens * threads <= 256 && tokens < 32 && T >= 8 * (int64_t)tokens * fg_num_sms()) tokens *= 2;
+    return dim3(threads, tokens);
+}
+
+// The same without whole warps: for kernels whose threads do not speak to each other.
+unsigned few_threads_for(int64_t n) { return n > 16 ? threads_for(n) : n > 8 ? 16 : 8; }
 
 bool aligned16(const void* p, int64_t stride_bytes) { return (uintptr_t)p % 16 == 0 && stride_bytes % 16 == 0; }
 
@@ -620,14 +648,14 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
     const SortArgs a{topk_ids, ids_are_i64, numel, num_experts, expert_map, expert_map_len, offs, row_of_slot, slot_of_row};
     const int64_t row_bytes = H * elem_bytes;
     const auto aligned = [&](int to) { return (uintptr_t)x % to == 0 && (uintptr_t)rows % to == 0 && ld_x * elem_bytes % to == 0 && row_bytes % to == 0; };
-    const bool vec = aligned(16);
+    const int unit = aligned(16) ? 16 : aligned(8) ? 8 : aligned(4) ? 4 : aligned(2) ? 2 : 1;
     const auto row_args = [&](int unit) {
-        return RowArgs{x, ld_x * elem_bytes / unit, scale, ld_scale, topk, numel, rows, (int)(row_bytes / unit), row_scale, (int)scale_cols};
+        return RowArgs{x, ld_x * elem_bytes / unit, scale, ld_scale, topk, T, numel, rows, (int)(row_bytes / unit), row_scale, (int)scale_cols};
     };
-    const RowArgs r = row_args(vec ? 16 : elem_bytes);
+    const RowArgs r = row_args(unit);
     const unsigned threads = threads_for(r.units);
     auto by_unit = [&](auto&& go) -> cudaError_t {
-        return vec ? go(uint4()) : elem_bytes == 4 ? go((unsigned int)0) : elem_bytes == 2 ? go((unsigned short)0) : go((unsigned char)0);
+        return unit == 16 ? go(uint4()) : unit == 8 ? go(uint2()) : unit == 4 ? go((unsigned int)0) : unit == 2 ? go((unsigned short)0) : go((unsigned char)0);
     };
     if (numel > 0 && one_launch(T, numel, row_bytes)) {
         // A row per CTA, four pieces per thread; with few tokens two pieces, and parts of a row until there are two CTAs per SM.
@@ -656,11 +684,18 @@ int fg_moe_permute(void* rows, float* row_scale, int32_t* offs, int32_t* row_of_
     // back because they may wait long, in the way of other streams).
     if (aligned(32)) {
         const RowArgs wide = row_args(32);
-        const unsigned block = wide.units >= 512 ? 512u : wide.units <= 32 ? 32u : (unsigned)(wide.units + 31) / 32 * 32;
-        FG_CUDA(fg_launch_when(true, permute_rows_kernel<Unit32>, (unsigned)T, block, 0, st, 1, a, ct, wide));
+        const dim3 block = wide.units > 256 ? dim3(wide.units >= 512 ? 512u : (unsigned)(wide.units + 31) / 32 * 32)
+                                            : block_of_tokens(few_threads_for(wide.units), T, row_bytes * (topk + 1));
+        FG_CUDA(fg_launch_when(true, block.y > 1 ? permute_rows_kernel<Unit32, true> : permute_rows_kernel<Unit32, false>,
+                               (unsigned)fg_cdiv(T, block.y), block, 0, st, 1, a, ct, wide));
         return FG_OK;
     }
-    FG_CUDA(by_unit([&](auto u) { return fg_launch_when(true, permute_rows_kernel<decltype(u)>, (unsigned)T, threads, 0, st, 1, a, ct, r); }));
+    const dim3 block = block_of_tokens(few_threads_for(fg_cdiv(r.units, 2)), T, row_bytes * (topk + 1));
+    FG_CUDA(by_unit([&](auto u) {
+        using U = decltype(u);
+        return fg_launch_when(true, block.y > 1 ? permute_rows_kernel<U, true> : permute_rows_kernel<U, false>, (unsigned)fg_cdiv(T, block.y),
+                              block, 0, st, 1, a, ct, r);
+    }));
     return FG_OK;
 }
 
@@ -674,7 +709,7 @@ int fg_moe_unpermute(void* out, const void* rows, const int32_t* row_of_slot, co
     FG_REQUIRE(out && (topk == 0 || (row_of_slot && (rows || n_rows == 0))), FG_ERR_INVALID_ARGUMENT, "null pointer");
     SumArgs a{};
     a.rows = rows; a.ld_rows = ld_rows; a.n_rows = n_rows; a.row_of_slot = row_of_slot; a.weights = weights; a.w_dtype = w_dtype;
-    a.ld_w = ld_w; a.topk = topk; a.H = H; a.out = out;
+    a.ld_w = ld_w; a.topk = topk; a.tokens = T; a.H = H; a.out = out;
     const int es = elem_size(dtype);
     const bool vec = aligned16(rows, ld_rows * es) && aligned16(out, H * es);
     const int slots = topk <= 2 ? 2 : topk <= 4 ? 4 : 8;  // at once
@@ -682,12 +717,17 @@ int fg_moe_unpermute(void* out, const void* rows, const int32_t* row_of_slot, co
     // Few tokens: their columns are spread over CTAs, until there are two CTAs per SM or a thread has one round.
     unsigned parts = 1;
     while (parts < 64 && T * parts < 2 * fg_num_sms() && parts * (int64_t)threads_for(pieces) < pieces) parts *= 2;
+    const dim3 block = parts > 1 ? dim3(threads_for(pieces)) : block_of_tokens(few_threads_for(pieces), T, H * es * (topk + 1));
     return by_type(dtype, [&](auto tag) -> int {
         using E = decltype(tag);
-        auto go = [&](auto kernel) { return fg_launch(kernel, dim3((unsigned)T, parts), threads_for(pieces), 0, (cudaStream_t)stream, 1, a); };
+        auto go = [&](auto kernel) { return fg_launch(kernel, dim3((unsigned)fg_cdiv(T, block.y), parts), block, 0, (cudaStream_t)stream, 1, a); };
+        auto of_slots = [&](auto v, auto k) {
+            constexpr int V = decltype(v)::value, K = decltype(k)::value;
+            return block.y > 1 ? go(unpermute_kernel<E, V, K, true>) : go(unpermute_kernel<E, V, K, false>);
+        };
         auto by_slots = [&](auto v) -> cudaError_t {
-            constexpr int V = decltype(v)::value;
-            return slots == 2 ? go(unpermute_kernel<E, V, 2>) : slots == 4 ? go(unpermute_kernel<E, V, 4>) : go(unpermute_kernel<E, V, 8>);
+            return slots == 2 ? of_slots(v, std::integral_constant<int, 2>())
+                 : slots == 4 ? of_slots(v, std::integral_constant<int, 4>()) : of_slots(v, std::integral_constant<int, 8>());
         };
         FG_CUDA(vec ? by_slots(std::integral_constant<int, 16 / sizeof(E)>()) : by_slots(std::integral_constant<int, 1>()));
         return FG_OK;
@@ -705,14 +745,18 @@ int fg_moe_unpermute_backward(void* d_rows, void* d_weights, const void* d_out, 
     FG_REQUIRE(row_of_slot && (H == 0 || d_out) && (!d_weights || rows || H == 0), FG_ERR_INVALID_ARGUMENT, "null pointer");
     SumArgs a{};
     a.rows = rows; a.ld_rows = ld_rows; a.n_rows = n_rows; a.row_of_slot = row_of_slot; a.weights = weights; a.w_dtype = w_dtype;
-    a.ld_w = ld_w; a.topk = topk; a.H = H; a.d_out = d_out; a.ld_d_out = ld_d_out; a.d_rows = d_rows; a.d_w = d_weights;
+    a.ld_w = ld_w; a.topk = topk; a.tokens = T; a.H = H; a.d_out = d_out; a.ld_d_out = ld_d_out; a.d_rows = d_rows; a.d_w = d_weights;
     const int es = elem_size(dtype);
     const bool vec = aligned16(d_out, ld_d_out * es) && (!d_weights || aligned16(rows, ld_rows * es)) && aligned16(d_rows, H * es);
     return by_type(dtype, [&](auto tag) -> int {
         using E = decltype(tag);
         constexpr int V = 16 / sizeof(E);
-        FG_CUDA(vec ? fg_launch(unpermute_backward_kernel<E, V>, (unsigned)T, threads_for(H / V), 0, (cudaStream_t)stream, 1, a)
-                    : fg_launch(unpermute_backward_kernel<E, 1>, (unsigned)T, threads_for(H), 0, (cudaStream_t)stream, 1, a));
+        const dim3 block = block_of_tokens(threads_for(vec ? H / V : H), T, H * es * (2 * topk + 1));
+        auto go = [&](auto kernel) { return fg_launch(kernel, (unsigned)fg_cdiv(T, block.y), block, 0, (cudaStream_t)stream, 1, a); };
+        auto of_values = [&](auto v) {
+            return block.y > 1 ? go(unpermute_backward_kernel<E, decltype(v)::value, true>) : go(unpermute_backward_kernel<E, decltype(v)::value, false>);
+        };
+        FG_CUDA(vec ? of_values(std::integral_constant<int, V>()) : of_values(std::integral_constant<int, 1>()));
         return FG_OK;
     });
 }

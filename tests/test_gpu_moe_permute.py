@@ -471,3 +471,29 @@ def test_inference_mode():
         plan2.row_of_slot.add_(0)  # an ordinary tensor in there
         assert rows2.is_inference() and plan2.row_of_slot.is_inference() and plan2.offs.is_inference()
     _same_plan([t.clone() for t in plan2], plan)
+
+
+@pytest.mark.parametrize("h", [8, 36, 38, 39, 200, 2040])
+@pytest.mark.parametrize("t,k,e", [(6, 3, 4), (300, 8, 64), (2501, 2, 9), (4800, 5, 320)])
+def test_int8_rows_of_any_alignment(t, k, e, h):
+    g = _gen(t + h)
+    ids = _ids(t, e, k, g)
+    ids[1] = e  # nowhere
+    wide = torch.randint(-128, 128, (t, 2064), device="cuda", generator=g, dtype=torch.int8)
+    scale = torch.rand(t, 3, device="cuda", generator=g)
+    want = _plan(ids, e)
+    for off in (0, 8, 4, 2, 1):
+        x = wide[:, off:off + h]
+        rows, row_scale, plan = flag_gems.moe_permute(x, ids, e, scale=scale)
+        _same_plan(plan, want)
+        _check_permuted(x, rows, plan, k)
+        valid = int(plan.offs[-1])
+        assert torch.equal(row_scale[:valid], scale[(plan.slot_of_row // k).long()][:valid]) and bool((row_scale[valid:] == 1.0).all())
+
+
+@pytest.mark.parametrize("t,k,e,h", [(2000, 40, 64, 8), (1185, 3, 5, 128), (4737, 2, 8, 100), (5000, 1, 16, 1024), (2400, 6, 64, 264), (9473, 1, 2, 72)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_many_narrow_rows(t, k, e, h, dtype):
+    test_permute(t, k, e, h, dtype)
+    test_unpermute(t, k, e, h, dtype)
+    test_gradients(t, k, e, h, dtype, torch.float32)
