@@ -91,6 +91,7 @@ struct FgSkinny {
     int sa_mode, sb_mode, out_dtype, bias_dtype, bias_after_round;
 };
 bool fg_int8_is_skinny(int64_t M);
+int64_t fg_int8_skinny_time(int64_t M, int64_t N, int64_t K);  // estimated, ns
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st);
 // The same with rows [offs[e - 1], offs[e]) of a times weight e of b [n_experts, N, K]; rows of c from offs[n_experts - 1] on
 // become zeros.  sa [M], sb [n_experts, N], bias rows bias_stride apart.
@@ -102,6 +103,7 @@ int fg_int8_skinny_grouped(const FgSkinny& p, const int32_t* offs, int n_experts
 struct FgInt8Tile {
     bool pair;
     int width;
+    int64_t time;  // ns
 };
 FgInt8Tile fg_int8_tile(int64_t blocks128, int64_t blocks256, int64_t N, int64_t K, int narrowest);
 

@@ -291,6 +291,78 @@ __device__ __forceinline__ TileCoord tile_coord(int t, int num_m, int num_n) {
     return tc;
 }
 
+// Split K, int8: adds up the partial tiles of 128 columns that the CTAs of the cluster have parked in shared memory and writes the results.
+// Whole numbers, so in any order.  A CTA finishes a share of the rows, a warp whole rows: first it adds the other slices' to
+// its own in place (nobody else reads those), then it scales them and writes each in one piece.  In two loops, because this
+// code runs once and what it waits for are its instructions too: with both unrolled over four rows 129 x 1000 x 8192 takes @ us, so @.
+// All threads of the cluster call it, also after a failed wait.
+template <int LD, int WARPS>
+__device__ __forceinline__ void add_int8_slices(const GemmParams& p, int* parked, const TileCoord tc, int width, bool has_tile) {
+    constexpr int ROWS = 4;  // whose slices are read at once
+    cg::cluster_group cluster = cg::this_cluster();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = 4 * lane;
+    const int slices = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int n = tc.n_blk * width + c, m0 = tc.m_blk * BLOCK_M;
+    const bool mine = has_tile && c < width && n < p.n_out;
+    float sb[4], bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int at = min(n + i, p.n_out - 1);
+        sb[i] = p.sb[p.sb_mode == FG_SCALE_VECTOR ? at : 0];
+        bias[i] = p.bias ? load_as_float(p.bias, p.bias_dtype, at) : 0.0f;
+    }
+    cluster.sync();  // all partial tiles are in shared memory
+    const int rows = (int)min((int64_t)BLOCK_M, p.M - m0), share = (rows + slices - 1) / slices;
+    const int first = rank * share + warp, last = min((rank + 1) * share, rows), esz = out_elem_size(p.out_dtype);
+    if (mine && first < last) {
+#pragma unroll 1
+        for (int r0 = first; r0 < last; r0 += ROWS * WARPS) {
+            int4 sum[ROWS];
+#pragma unroll
+            for (int b = 0; b < ROWS; ++b) sum[b] = make_int4(0, 0, 0, 0);
+#pragma unroll 1
+            for (int q = 0; q < slices; ++q) {
+                const int* part = cluster.map_shared_rank(parked, q) + c;
+#pragma unroll
+                for (int b = 0; b < ROWS; ++b) {
+                    const int4 x = *reinterpret_cast<const int4*>(part + min(r0 + b * WARPS, last - 1) * LD);
+                    sum[b].x += x.x;
+                    sum[b].y += x.y;
+                    sum[b].z += x.z;
+                    sum[b].w += x.w;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < ROWS; ++b)
+                if (r0 + b * WARPS < last) *reinterpret_cast<int4*>(parked + (r0 + b * WARPS) * LD + c) = sum[b];
+        }
+#pragma unroll 1
+        for (int r = first; r < last; r += WARPS) {
+            const int4 sum = *reinterpret_cast<const int4*>(parked + r * LD + c);
+            const float sa = p.sa[p.sa_mode == FG_SCALE_VECTOR ? m0 + r : 0];
+            float v[4] = {sb[0] * (sa * __int2float_rn(sum.x)), sb[1] * (sa * __int2float_rn(sum.y)),
+                          sb[2] * (sa * __int2float_rn(sum.z)), sb[3] * (sa * __int2float_rn(sum.w))};
+            if (p.bias) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (p.bias_after_round ? round_through(v[i], p.out_dtype) : v[i]) + bias[i];
+            }
+            uint8_t* out = reinterpret_cast<uint8_t*>(p.c) + ((m0 + r) * p.ld_c + n) * esz;
+            if (p.c_vec_ok && n + 4 <= p.n_out) {
+                if (esz == 4) *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+                else *reinterpret_cast<uint2*>(out) = make_uint2(fg_pair_of(v[0], v[1], p.out_dtype), fg_pair_of(v[2], v[3], p.out_dtype));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (n + i >= p.n_out) break;
+                    if (esz == 4) reinterpret_cast<float*>(out)[i] = v[i];
+                    else reinterpret_cast<uint16_t*>(out)[i] = (uint16_t)fg_pair_of(v[i], 0.0f, p.out_dtype);
+                }
+            }
+        }
+    }
+    cluster.sync();  // nobody leaves while a peer may still read its partial tile
+}
+
 // SPLITK: the CTAs of one thread-block cluster share an output tile and split its K range; each
 // leaves its fp32 partial tile in its own shared memory and the cluster adds them up through
 // distributed shared memory (no global scratch, no atomics).  For decode-sized M, where there are
@@ -310,8 +382,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     static_assert(!ASTORE || (BLOCK_SCALED && !SPLITK), "the store warp serves the block-scaled tiles");
     constexpr bool INT8 = OPK == 1;
     static_assert(!BY_ROWS || (INT8 && !FUSE_SILU), "built for int8 products");
-    // int8 products of up to 128 rows are int8_skinny.cu's; 16-bit operands serve the grouped tiles
-    static_assert(OPK == 0 || (!BLOCK_SCALED && !SPLITK && !SMALL_A), "these are built for e4m3 operands");
+    // 16-bit operands serve the grouped tiles
+    static_assert(OPK == 0 || (!BLOCK_SCALED && !SMALL_A && !(SPLITK && (OPK > 1 || BN != 128))), "these are built for e4m3 operands");
     // accumulator word -> fp32
     auto acc_f = [](uint32_t raw) -> float {
         if constexpr (INT8) return __int2float_rn((int)raw);
@@ -1135,7 +1207,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 #endif
     }
 
-    if constexpr (SPLITK) {
+    if constexpr (SPLITK && INT8) {
+        add_int8_slices<BN + 4, C::THREADS / 32>(p, reinterpret_cast<int*>(smem), tile_coord(tile_first, num_m, num_n), OUT_TILE_N,
+                                                 tile_first < num_tiles);
+    } else if constexpr (SPLITK) {
         // ------------------------- cluster reduction of the K slices ---------------------------
         // Every thread of every CTA of the cluster reaches both syncs, also after a failed wait.
         cg::cluster_group cluster = cg::this_cluster();
@@ -1243,7 +1318,7 @@ int fg_byte_map(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint
 namespace {
 
 // How many clusters of `slices` CTAs of the split-K kernel fit on the device at once (cached).
-template <int BN, bool BS>
+template <int BN, bool BS, int OPK = 0>
 int max_resident_clusters(int slices) {
     static int table[64][9];
     static std::mutex mu;
@@ -1251,7 +1326,7 @@ int max_resident_clusters(int slices) {
     int* cache = table[fg_device_index()];
     if (cache[slices]) return cache[slices];
     using C = Cfg<BN, false>;
-    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true>;
+    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true, false, false, OPK>;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(slices * 64), 1, 1);
@@ -1273,11 +1348,11 @@ int max_resident_clusters(int slices) {
     return n;
 }
 
-template <int BN, bool BS>
+template <int BN, bool BS, int OPK = 0>
 int launch_splitk(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, int tiles, int slices,
                   cudaStream_t st) {
     using C = Cfg<BN, false>;
-    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true>;
+    auto kernel = gemm_fp8_kernel<BN, BS, false, false, true, false, false, OPK>;
     static bool attr_done[64];
     static std::mutex mu;
     {
@@ -1290,6 +1365,31 @@ int launch_splitk(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams
     }
     FG_CUDA(fg_launch(kernel, (unsigned)(tiles * slices), C::THREADS, C::SMEM_BYTES, st, (unsigned)slices, ta, tb, p));
     return FG_OK;
+}
+
+// int8 products with few tiles and a long K: the width of a tile and the slices of K (a cluster's CTAs, one wave of them) with the least
+// estimated time, if that is below 95 % of `least` ns, the time of a form without; slices 1 otherwise.  A block of K costs what it
+// does in fg_int8_tile; the rest is the launch of clusters and the sum over their shared memory.  Measured, without / split: 129 x
+// 1000 x 8192 22.1 / 12.3 us (64 wide, 4 slices), 129 x 4096 x 14336 37.4 / 28.3 (128, 2), 128 x 4096 x 14336 24.2 / 20.8 (128, 4),
+// 256 x 2112 x 7168 19.9 / 16.5 (128, 3); 129 x 4096 x 4096 13.6 / 14.8, which stays whole.
+struct Int8Split {
+    int width, slices;
+};
+Int8Split int8_split(int64_t M, int64_t N, int64_t K, int64_t least) {
+    const int64_t k_blocks = fg_cdiv(K, BLOCK_K);
+    Int8Split best{0, 1};
+    least = least * 95 / 100;
+    for (int width = 64; width <= 128; width += 32) {
+        const int64_t tiles = fg_cdiv(M, BLOCK_M) * fg_cdiv(N, width);
+        for (int slices = 2; slices <= 8 && tiles * slices <= fg_num_sms(); ++slices) {
+            const int64_t per = fg_cdiv(k_blocks, slices), time = 5500 + 400 * slices + 20 * width + per * (285 + 55 * (width - 64) / 64);
+            if (per < 2 || (slices - 1) * per >= k_blocks || time >= least) continue;
+            if (max_resident_clusters<128, false, 1>(slices) < tiles) continue;
+            least = time;
+            best = Int8Split{width, slices};
+        }
+    }
+    return best;
 }
 
 // Whether a product is launched while its predecessor drains.  That saves ~2 us, but the CTAs then land on the
@@ -1441,6 +1541,13 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
         int8_pair = t.pair;
         bn = t.width > 128 || t.pair ? 256 : t.width > 64 ? 128 : 64;
         p.tile_n = t.width;
+        const Int8Split split = int8_split(p.M, p.n_out, p.K, fg_int8_is_skinny(p.M) ? fg_int8_skinny_time(p.M, p.n_out, p.K) : t.time);
+        if (split.slices > 1) {
+            int8_pair = false;
+            bn = 128;
+            p.tile_n = split.width;
+            k_slices = split.slices;
+        }
     } else if (want_width > 0) {
         bn = want_width > 128 || grouped_pair ? 256 : 128;
         p.tile_n = want_width;
@@ -1460,9 +1567,9 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
                   (uint64_t)ld_b * (uint64_t)p.N, (uint32_t)(fuse_silu ? bn / 2 : pair ? p.tile_n / 2 : p.tile_n), 3);
     if (rc != FG_OK) return rc;
     // int8 results of 32 bits, or in rows that are not aligned, are written row by row (store_rows.cuh), and so are those of more than
-    // one wave of tiles, where that takes fewer instructions from the next tile's: 2048 x 7168 x 2048 29.4 us (30.9), 3859 x 6144 x
-    // 4096 70.4 (73.4).  A single wave waits for the larger code at its end: 129 x 7168 x 2048 11.1 us, without 10.7.
-    const bool by_rows = p.int8 == 1 && !fuse_silu && (esz == 4 || !p.c_vec_ok || (!p.grouped && tiles > sms));
+    // one wave of CTA pairs, where that takes fewer instructions from the next tile's: 2048 x 7168 x 2048 29.4 us (30.9), 3859 x 6144
+    // x 4096 70.4 (73.4).  Elsewhere the larger code costs more at the end: 129 x 7168 x 2048 11.1 us (10.7), 200 x 24576 x 1536 17.8 (17.3).
+    const bool by_rows = p.int8 == 1 && !fuse_silu && (esz == 4 || !p.c_vec_ok || (int8_pair && pair_tiles > sms / 2));
     if (pair) {
         FG_REQUIRE(pair_tiles < (1ll << 30), FG_ERR_UNSUPPORTED, "too many tiles");
         auto by_kind = [&](auto silu_tag) -> int {
@@ -1485,6 +1592,7 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
     if (p.int8) {
         FG_REQUIRE(!block_scaled && (p.int8 == 1 || p.grouped), FG_ERR_UNSUPPORTED,
                    "int8 operands take no block scales, and 16-bit operands are built for the grouped expert GEMMs");
+        if (k_slices > 1) return launch_splitk<128, false, 1>(ta, tb, p, t, k_slices, st);
         if (bn == 64) return by_rows ? launch_inst<64, false, false, false, false, 1, true>(ta, tb, p, t, st)
                                      : launch_inst<64, false, false, false, false, 1>(ta, tb, p, t, st);
         auto by_kind = [&](auto bn_tag, auto silu_tag) -> int {
@@ -1576,8 +1684,9 @@ int scaled_mm_common(int operand, void* c, const void* a, const void* b, const f
     if (operand == 1 && fg_int8_is_skinny(M)) {
         const int rc = check_operands(a, b, K, ld_a, ld_b);
         if (rc != FG_OK) return rc;
-        return fg_int8_skinny(FgSkinny{c, (const int8_t*)a, (const int8_t*)b, sa, sb, bias, M, N, K, ld_a, ld_b, ld_c, sa_mode, sb_mode,
-                                       out_dtype, bias_dtype, bias_after_round}, (cudaStream_t)stream);
+        if (int8_split(M, N, K, fg_int8_skinny_time(M, N, K)).slices == 1)
+            return fg_int8_skinny(FgSkinny{c, (const int8_t*)a, (const int8_t*)b, sa, sb, bias, M, N, K, ld_a, ld_b, ld_c, sa_mode, sb_mode,
+                                           out_dtype, bias_dtype, bias_after_round}, (cudaStream_t)stream);
     }
     return launch_gemm(p, a, M, ld_a, b, 1, ld_b, false, false, (cudaStream_t)stream);
 }
@@ -1685,14 +1794,14 @@ int fg_grouped_gemm_fp8_bias(void* c, const void* a, const void* w, const float*
 FgInt8Tile fg_int8_tile(int64_t blocks128, int64_t blocks256, int64_t N, int64_t K, int narrowest) {
     const int sms = fg_num_sms();
     const int64_t k_blocks = fg_cdiv(K, BLOCK_K);
-    FgInt8Tile best{false, 256};
+    FgInt8Tile best{false, 256, 0};
     int64_t least = INT64_MAX;
     auto offer = [&](bool pair, int width, int64_t start, int64_t per_block) {
         const int64_t tiles = (pair ? blocks256 : blocks128) * fg_cdiv(N, width);
         const int64_t time = start + fg_cdiv(tiles, pair ? sms / 2 : sms) * k_blocks * per_block;
         if (time < least) {
             least = time;
-            best = FgInt8Tile{pair, width};
+            best = FgInt8Tile{pair, width, time};
         }
     };
     for (int width = 256; width >= 96; width -= 32) offer(false, width, 4000, 290 + 130 * width / 256);

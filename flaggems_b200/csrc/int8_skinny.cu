@@ -89,13 +89,13 @@ __device__ void drain(uint64_t* full_bar, int stages, int issued) {
         mbar_wait(&full_bar[j % stages], (uint32_t)(j / stages) & 1u, &alone, nullptr, 0, 100000000ull);
 }
 
-// 32 values to a 16-byte boundary.
-__device__ __forceinline__ void store_row(uint8_t* to, const float (&v)[32], int dtype) {
+// `cols` values, a multiple of eight, to a 16-byte boundary.
+__device__ __forceinline__ void store_row(uint8_t* to, const float (&v)[32], int cols, int dtype) {
     uint4* o = reinterpret_cast<uint4*>(to);
     if (dtype == FG_DTYPE_F32) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            o[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+            if (4 * i < cols) o[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
         return;
     }
 #pragma unroll
@@ -103,7 +103,7 @@ __device__ __forceinline__ void store_row(uint8_t* to, const float (&v)[32], int
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = fg_pair_of(v[8 * i + 2 * j], v[8 * i + 2 * j + 1], dtype);
-        o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (8 * i < cols) o[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -474,8 +474,8 @@ __global__ void __launch_bounds__(256, 1) int8_stream_kernel(const __grid_consta
                 }
                 // Whole pieces of aligned rows by their own lanes: there is little to write, and its end is waited for (64 x 9472 x 4096
                 // 10.8 us, 11.4 through shared memory; 64 x 9471 12.3, by their own lanes 17).
-                if (a.c_align == 16 && cols == 32) {
-                    if (mine) store_row(out + (n0 + c) * esz, v, p.out_dtype);
+                if (a.c_align == 16 && cols % 8 == 0) {
+                    if (mine) store_row(out + (n0 + c) * esz, v, cols, p.out_dtype);
                 } else {
                     fg_store_rows(staging, lane, v, rows, p.ld_c * esz, (n0 + c) * esz, cols, p.out_dtype, a.c_align);
                 }
@@ -597,7 +597,9 @@ int launch_tensor_memory(StreamArgs& a, cudaStream_t st) {
     a.token_rows = (int)((a.p.M + 7) / 8 * 8);
     a.c_align = fg_row_align(a.p.c, a.p.ld_c * (a.p.out_dtype == FG_DTYPE_F32 ? 4 : 2));
     const int rows = a.rows + a.token_rows;
-    return rows <= 96 ? launch_stream<4>(a, st) : rows <= 192 ? launch_stream<2>(a, st) : launch_stream<1>(a, st);
+    // Four blocks of K per stage while three such stages fit: 4096 x 14336 with 80 tokens 21.2 us, 24.5 with two blocks.  Three blocks
+    // take 11.4 us where two take 10.8 (9472 x 4096 with 65).
+    return rows <= 128 ? launch_stream<4>(a, st) : rows <= 192 ? launch_stream<2>(a, st) : launch_stream<1>(a, st);
 }
 
 // Rows per group: as few rounds of groups as their height allows, and in those all groups of one height.
@@ -606,9 +608,24 @@ int group_rows(int64_t N) {
     return (int)(fg_cdiv(fg_cdiv(N, rounds * fg_num_sms()), 16) * 16);
 }
 
+// A tcgen05 instruction takes 64 cycles for its 128 rows of tokens however few they are and however low the group is, 142 ns
+// per block of K, where the registers' instructions take what tokens and rows cost; those run out above (0.4 PFLOP/s).
+// Measured, registers / TMEM: 2112 x 7168 5.6 / 10.7 us with 16 tokens, 7.2 / 10.6 with 32; 6144 x 4096 7.6 / 8.9 with 16,
+// 9.5 / 8.9 with 32; 24576 x 7168 33.3 / 33.1 and 39.1 / 33.2; 4096 x 14336 15.7 / 20.2 with 32, 21.8 / 19.7 with 33.
+bool in_registers(int64_t M, int rows) { return M <= 16 || (M <= 32 && rows <= 32); }
+
 }  // namespace
 
 bool fg_int8_is_skinny(int64_t M) { return M <= MAX_TOKENS; }
+
+// Where the stream of the weight does not bound it: a block of K takes what the instruction and the ring take, or the bytes that an SM
+// takes in, 113 per ns.
+int64_t fg_int8_skinny_time(int64_t M, int64_t N, int64_t K) {
+    const int rows = group_rows(N);
+    if (in_registers(M, rows)) return 0;  // nothing is faster
+    const int64_t bytes = (rows + fg_cdiv(M, 8) * 8) * BLOCK_K, ring = bytes <= 128 * BLOCK_K ? 150 : 178;
+    return 3000 + fg_cdiv(fg_cdiv(N, rows), fg_num_sms()) * fg_cdiv(K, BLOCK_K) * (bytes / 113 > ring ? bytes / 113 : ring);
+}
 
 int fg_int8_skinny(const FgSkinny& p, cudaStream_t st) {
     FG_REQUIRE(p.M > 0 && p.N > 0 && p.M <= MAX_TOKENS && p.K > 0 && p.K % 16 == 0, FG_ERR_UNSUPPORTED, "bad sizes");
@@ -617,12 +634,7 @@ int fg_int8_skinny(const FgSkinny& p, cudaStream_t st) {
     a.status = fg_status_word_device_ptr();
     a.rows = group_rows(p.N);
     a.groups = (int)fg_cdiv(p.N, a.rows);
-    // A tcgen05 instruction takes 64 cycles for its 128 rows of tokens however few they are and however low the group is, 142 ns
-    // per block of K, where the registers' instructions take what tokens and rows cost; those run out above (0.4 PFLOP/s).
-    // Measured, registers / TMEM: 2112 x 7168 5.6 / 10.7 us with 16 tokens, 7.2 / 10.6 with 32; 6144 x 4096 7.6 / 8.9 with 16,
-    // 9.5 / 8.9 with 32; 24576 x 7168 33.3 / 33.1 and 39.1 / 33.2; 4096 x 14336 15.7 / 20.2 with 32, 21.8 / 19.7 with 33.
-    const bool registers = p.M <= 16 || (p.M <= 32 && a.rows <= 32);
-    return registers ? launch_registers<false>(a, st) : launch_tensor_memory(a, st);
+    return in_registers(p.M, a.rows) ? launch_registers<false>(a, st) : launch_tensor_memory(a, st);
 }
 
 // The same for experts: rows [offs[e - 1], offs[e]) of up to 16 in all times weight e.  One launch without tables of tiles, and groups

@@ -115,6 +115,22 @@ def test_types_and_bias(m, out, bias):
     _check(got, _definition(a, b, a_s, b_s), c)
 
 
+@pytest.mark.parametrize("m,n,k", [(100, 1000, 8192), (128, 4096, 14336), (127, 999, 8208), (129, 1000, 8192), (200, 1001, 8208), (256, 2112, 7168),
+                                   (257, 2112, 7184), (300, 1002, 16384), (384, 1000, 8192), (500, 130, 7168), (1000, 64, 7168), (70, 16, 65536)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("bias", [None, torch.float32])
+def test_long_rows_and_narrow_weights(m, n, k, out, bias):
+    """Few tiles, so that K is split over a cluster."""
+    a, b, a_s, b_s, g = _operands(m, n, k, seed=m)
+    c = None if bias is None else torch.randn(n, device="cuda", generator=g).to(bias)
+    kept = [flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, c, out) for _ in range(3)]
+    _check(kept[0], _definition(a, b, a_s, b_s), c)
+    assert torch.equal(kept[0], kept[1]) and torch.equal(kept[0], kept[2])
+    one = torch.tensor([0.01], device="cuda")
+    _check(flag_gems.w8a8_int8_matmul(a, b, one, one, c, out), _definition(a, b, one.expand(m), one.expand(n)), c)
+    assert _cabi.device_status() == 0
+
+
 @pytest.mark.parametrize("m", [1, 3, 200])
 def test_scale_shapes(m):
     a, b, a_s, b_s, _ = _operands(m, 96, 64)
@@ -153,7 +169,7 @@ def test_strides_and_alignment():
     assert torch.equal(flag_gems.w8a8_int8_matmul(a, b, a_s, every_other), want)
 
 
-@pytest.mark.parametrize("m", [1, 16, 100, 300])
+@pytest.mark.parametrize("m", [1, 16, 100, 129, 300])
 def test_sums_at_the_edge_of_32_bits(m):
     """K as large as it may be with every product 2^14: the largest sum is 2^31 - 2^18."""
     k = 131056
@@ -212,7 +228,7 @@ def test_cutlass_scaled_mm(m, n, k, bias, out):
 @pytest.mark.parametrize("off", [0, 1, 2, 8])
 def test_results_between_others(m, n, out, off):
     """Rows that begin at any value, in a wider matrix whose other values stay as they are."""
-    a, b, a_s, b_s, _ = _operands(m, n, 272, seed=n)
+    a, b, a_s, b_s, _ = _operands(m, n, 272 if m != 131 else 8208, seed=n)
     wide = torch.full((m, (n + off + 31) // 16 * 16), 7.0, dtype=out, device="cuda")
     flag_gems.cutlass_scaled_mm(wide[:, off:off + n], a, b.t(), a_s, b_s)
     _check(wide[:, off:off + n], _definition(a, b, a_s, b_s))
