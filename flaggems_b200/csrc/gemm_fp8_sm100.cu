@@ -365,7 +365,7 @@ __device__ __forceinline__ void add_int8_slices(const GemmParams& p, int* parked
 }
 
 // SPLITK: the CTAs of one thread-block cluster share an output tile and split its K range; each
-// leaves its fp32 partial tile in its own shared memory and the cluster adds them up through
+// leaves its partial tile (fp32, int8: 32-bit) in its own shared memory and the cluster adds them up through
 // distributed shared memory (no global scratch, no atomics).  For decode-sized M, where there are
 // fewer tiles than SMs and the job is to pull the weights from HBM with every SM.
 // OPK (operand kind): 0 = e4m3 (kind::f8f6f4); 1 = signed 8-bit integers with 32-bit integer accumulators

@@ -227,11 +227,11 @@ __global__ void __launch_bounds__(256) scan_chunks_kernel(SortArgs s, ChunkTable
     }
 }
 
-// Many slots, third launch, one CTA per token, or per several (threadIdx.y) of narrow rows: a row is read once and written slot after slot.  Bound by the writes, which
-// are topk times the reads, and by the rate of a copy.  Few registers (and so many CTAs, a row each, under way) matter more
-// than pieces per thread, and accesses of 32 bytes more than those of 16: 8192 x 8 rows of 14336 bytes take 164 us (6.4 TB/s
-// of the 6.6 of a copy), 178 with two pieces of 16 bytes per thread; rows of 7168 bytes 84, 88, and 98 with four pieces and the
-// slots' rows in registers, 91-97 as bulk copies through a ring in shared memory.
+// Many slots, third launch, one CTA per token, or per several (threadIdx.y) of narrow rows: a row is read once and written slot
+// after slot.  Bound by the writes, which are topk times the reads, and by the rate of a copy.  Few registers (and so many CTAs,
+// a row each, under way) matter more than pieces per thread, and accesses of 32 bytes more than those of 16: 8192 x 8 rows of
+// 14336 bytes take 164 us (6.4 TB/s of the 6.6 of a copy), 178 with two pieces of 16 bytes per thread; rows of 7168 bytes 84,
+// 88, and 98 with four pieces and the slots' rows in registers, 91-97 as bulk copies through a ring in shared memory.
 // UNIT: the bytes of a load, the most that everything is aligned to.
 template <typename UNIT, bool SHARED>
 __global__ void __launch_bounds__(512) permute_rows_kernel(SortArgs s, ChunkTable ct, RowArgs a) {
@@ -424,8 +424,8 @@ __device__ __forceinline__ void load_slots(const SumArgs& a, int64_t t, int k0, 
         if (row[k] < 0 || row[k] >= a.n_rows) row[k] = -1;
 }
 
-// One CTA per token and per part of its columns (blockIdx.y), or per several tokens (threadIdx.y), sums in fp32 in slot order.  A thread has K slots
-// of U pieces in flight, eight loads whatever the number of slots.
+// One CTA per token and per part of its columns (blockIdx.y), or per several tokens (threadIdx.y), sums in fp32 in slot order.
+// A thread has K slots of U pieces in flight, eight loads whatever the number of slots.
 template <typename T, int V, int K, bool SHARED>
 __global__ void __launch_bounds__(256) unpermute_kernel(SumArgs a) {
     fg_pdl_wait();
@@ -474,11 +474,11 @@ __global__ void __launch_bounds__(256) unpermute_kernel(SumArgs a) {
     }
 }
 
-// One CTA per token, or per several (threadIdx.y, whole warps each): d_out[t] times the weight into the gradient of every row of the token, and its product with
-// the row into the gradient of the weight, slot after slot.  d_out is read once where a row is up to four pieces per
-// thread (16 KB), everything else is read and written once; the products are summed in a fixed order: a thread's columns, the
-// lanes, the warps.  Bound by HBM: 8192 x 8 bf16 rows of 7168 (2.0 GB) take 307 us, 6.5 TB/s, which is the rate of a
-// copy.  More slots in flight per thread cost registers and with them CTAs (404 us with two slots at once); streaming
+// One CTA per token, or per several (threadIdx.y, whole warps each): d_out[t] times the weight into the gradient of every row of
+// the token, and its product with the row into the gradient of the weight, slot after slot. d_out is read once where a row is up
+// to four pieces per thread (16 KB), everything else is read and written once; the products are summed in a fixed order: a
+// thread's columns, the lanes, the warps.  Bound by HBM: 8192 x 8 bf16 rows of 7168 (2.0 GB) take 307 us, 6.5 TB/s, which is the
+// rate of a copy.  More slots in flight per thread cost registers and with them CTAs (404 us with two slots at once); streaming
 // loads and stores (.cs) take 315.
 template <typename T, int V, bool SHARED>
 __global__ void __launch_bounds__(256, 4) unpermute_backward_kernel(SumArgs a) {

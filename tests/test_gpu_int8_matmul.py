@@ -131,6 +131,47 @@ def test_long_rows_and_narrow_weights(m, n, k, out, bias):
     assert _cabi.device_status() == 0
 
 
+@pytest.mark.parametrize("m,n,k", [(128, 1000, 8192), (300, 576, 7168)])
+def test_split_products_in_streams_and_graphs(m, n, k):
+    """Operands that the kernel before writes, two streams at once, and two captured graphs replayed with other operands."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = torch.randn(m, k, device="cuda", generator=g).bfloat16(), torch.randn(n, k, device="cuda", generator=g).bfloat16()
+
+    def layer():
+        a, a_s = flag_gems.per_token_quant_int8(x)
+        b, b_s = flag_gems.per_token_quant_int8(w)
+        return a, b, a_s, b_s, flag_gems.w8a8_int8_matmul(a, b, a_s, b_s)
+
+    def check(got):
+        _check(got[4], _definition(*got[:4]))
+
+    check(layer())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(layer())
+    torch.cuda.synchronize()
+    for r in got:
+        check(r)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer()
+        graphs.append((graph, out))
+    for _ in range(3):
+        x.copy_(x.roll(1, 1) * 1.5)
+        w.copy_(w.roll(5, 0))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            check(out)
+    assert _cabi.device_status() == 0
+
+
 @pytest.mark.parametrize("m", [1, 3, 200])
 def test_scale_shapes(m):
     a, b, a_s, b_s, _ = _operands(m, 96, 64)
