@@ -1553,7 +1553,7 @@ int launch_gemm(GemmParams& p, const void* a, int64_t a_rows, int64_t ld_a, cons
         bn = want_width > 128 || grouped_pair ? 256 : 128;
         p.tile_n = want_width;
     }
-    const int64_t pair_tiles = fg_cdiv(p.M, 2 * BLOCK_M) * fg_cdiv(p.n_out, fuse_silu ? 128 : int8_pair ? p.tile_n : 256);
+    const int64_t pair_tiles = fg_cdiv(p.M, 2 * BLOCK_M) * fg_cdiv(p.n_out, p.tile_n);
     const bool pair = int8_pair || grouped_pair || (p.int8 == 0 && !p.grouped && !fuse_silu && !block_scaled && bn == 256 && k_slices == 1 &&
                                        pair_tiles >= 3 * (int64_t)(sms / 2) && pair_tiles < (1ll << 30) && pair_enabled());
     const int64_t tiles = m_tiles * fg_cdiv(p.n_out, p.tile_n);

@@ -4,6 +4,8 @@ Tolerances count roundings.  The sum of products is a whole number, exact in 32 
 multiply it: three relative errors of 2^-24.  The bias joins with one rounding of the result, the cast adds half a step
 of the output type (fp16 results below its normal range: half of 2^-24).
 """
+import ctypes
+
 import pytest
 import torch
 
@@ -381,6 +383,41 @@ def test_grouped_tiles_of_every_width(sizes, n):
     got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs, bias, torch.float16)
     _check(got[:-5], want[:-5], bias[group])
     assert not got[-5:].any()
+
+
+class _KernelNode(ctypes.Structure):
+    """CUDA_KERNEL_NODE_PARAMS of the driver API."""
+    _fields_ = [("func", ctypes.c_void_p), ("grid", ctypes.c_uint * 3), ("block", ctypes.c_uint * 3), ("shared", ctypes.c_uint),
+                ("params", ctypes.c_void_p), ("extra", ctypes.c_void_p), ("kern", ctypes.c_void_p), ("ctx", ctypes.c_void_p)]
+
+
+def _grids(call):
+    """CTAs of the kernels that ``call`` launches, from a captured graph that never runs."""
+    call()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    cu, raw, n = ctypes.CDLL("libcuda.so.1"), ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t()
+    assert cu.cuGraphGetNodes(raw, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert cu.cuGraphGetNodes(raw, nodes, ctypes.byref(n)) == 0
+    grids = []
+    for node in nodes:
+        kind, params = ctypes.c_int(), _KernelNode()
+        assert cu.cuGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        if kind.value == 0:
+            assert cu.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(node), ctypes.byref(params)) == 0
+            grids.append(params.grid[0] * params.grid[1] * params.grid[2])
+    return grids
+
+
+# rows of the groups, and the tiles of CTA pairs that their products take: 128, 128 and 192 columns
+@pytest.mark.parametrize("sizes,n,k,tiles", [([207, 207], 4096, 7168, 64), ([503], 4096, 7168, 64), ([540], 4096, 14336, 66)])
+def test_grouped_pairs_have_a_cta_pair_for_every_tile(sizes, n, k, tiles):
+    a, b, a_s, b_s, offs, _ = _grouped(sizes, n, k)
+    pairs = torch.cuda.get_device_properties(0).multi_processor_count // 2
+    assert max(_grids(lambda: flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs))) >= 2 * min(tiles, pairs)
+    _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, offs), _grouped_definition(a, b, a_s, b_s, offs))
 
 
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
