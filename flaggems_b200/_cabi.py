@@ -184,6 +184,11 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def row_stride(t):
+    """Elements between the rows of a 2-D tensor; a single row has any stride and counts as the row's length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def stream_ptr(device=None):
     return torch.cuda.current_stream(device).cuda_stream
 

@@ -75,13 +75,14 @@ at::Tensor empty(at::IntArrayRef sizes, ScalarType dtype, const at::Tensor& like
 
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
-// Rows of a tensor seen as [rows, last dimension]: true when one stride addresses them all.
+// Rows of a tensor seen as [rows, last dimension]: true when one stride addresses them all.  A single row has any stride; it
+// counts as the row's length, which the kernels' checks of alignment take.
 bool as_rows(const at::Tensor& t, int64_t* rows, int64_t* cols, int64_t* ld) {
     if (t.dim() < 1 || t.numel() == 0) return false;
     *cols = t.size(-1);
     *rows = t.numel() / *cols;
     if (t.dim() == 2) {
-        *ld = t.stride(0);
+        *ld = *rows > 1 ? t.stride(0) : *cols;
         return t.stride(1) == 1;
     }
     *ld = *cols;

@@ -70,7 +70,7 @@ def _per_token_quant(x, row_index=None, index_div=1, index_limit=0, n_rows_dev=N
         _cabi.check(
             _cabi.lib().fg_per_token_quant_fp8(
                 _cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], _cabi.ptr(q), _cabi.ptr(s), rows, k,
-                x2.stride(0), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev),
+                _cabi.row_stride(x2), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev),
                 _cabi.stream_ptr(x.device),
             )
         )
@@ -89,7 +89,7 @@ def _per_token_quant_int8(x, row_index=None, index_div=1, index_limit=0, n_rows_
         _cabi.check(
             _cabi.lib().fg_per_token_quant_int8(
                 _cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], _cabi.ptr(q), _cabi.ptr(s), rows, k,
-                x2.stride(0), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev),
+                _cabi.row_stride(x2), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev),
                 _cabi.stream_ptr(x.device),
             )
         )
@@ -116,7 +116,7 @@ def _group_quant(x, group, row_index=None, index_div=1, index_limit=0, n_rows_de
         _cabi.check(
             _cabi.lib().fg_per_token_group_quant_fp8_gather(
                 _cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], _cabi.ptr(q), _cabi.ptr(s), rows, k, group,
-                x2.stride(0), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev),
+                _cabi.row_stride(x2), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev),
                 _cabi.stream_ptr(x.device),
             )
         )
@@ -155,12 +155,12 @@ def _per_tensor_quant(x, scale=None, row_index=None, index_div=1, index_limit=0,
         s_in = torch.zeros(1, dtype=torch.float32, device=x.device)
         s_out, dynamic = torch.empty(1, dtype=torch.float32, device=x.device), 1
         if x2.shape[0] and k:
-            _cabi.check(L.fg_abs_max(_cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], x2.shape[0], k, x2.stride(0),
+            _cabi.check(L.fg_abs_max(_cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], x2.shape[0], k, _cabi.row_stride(x2),
                                      _cabi.ptr(amax_rows_dev), _cabi.ptr(s_in), st))
     if rows and k:
         _cabi.check(L.fg_per_tensor_quant_fp8(
             _cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], _cabi.ptr(q), _cabi.ptr(s_in), dynamic, _cabi.ptr(s_out),
-            rows, k, x2.stride(0), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev), st))
+            rows, k, _cabi.row_stride(x2), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev), st))
     return q, s_out
 
 

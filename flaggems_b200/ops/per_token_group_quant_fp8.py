@@ -49,11 +49,8 @@ def per_token_group_quant_fp8(
         return x_q, x_s
 
     # Rows are addressed through one stride: collapse the leading dimensions.
-    if x.dim() == 2:
-        x2, ld_x = x, x.stride(0)
-    else:
-        x2 = x.reshape(-1, k)  # a view whenever the leading dims are collapsible
-        ld_x = x2.stride(0)
+    x2 = x.reshape(-1, k)  # a view whenever the leading dims are collapsible
+    ld_x = _cabi.row_stride(x2)
     m = x2.shape[0]
     if column_major_scales:
         assert x.dim() == 2, "column-major scales are defined for 2-D inputs"

@@ -43,7 +43,7 @@ def per_token_quant_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         _cabi.check(
             _cabi.lib().fg_per_token_quant_int8(
                 _cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], _cabi.ptr(q), _cabi.ptr(s), m, k,
-                x2.stride(0) if m > 1 else k, k, None, 1, 0, None, _cabi.stream_ptr(x.device),
+                _cabi.row_stride(x2), k, None, 1, 0, None, _cabi.stream_ptr(x.device),
             )
         )
     return q, s

@@ -140,3 +140,18 @@ def test_a_flag_without_a_truth_value_raises_its_own_error():
                  lambda: flag_gems.topk_softmax(*_topk(torch.int32), x[:5, :16].contiguous(), both)):
         with pytest.raises(RuntimeError, match="ambiguous"):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_single_row_may_have_any_stride(dtype, monkeypatch):
+    scale = torch.full((1,), 0.01, device="cuda")
+    quantisers = [flag_gems.per_token_quant_int8, lambda x: flag_gems.moe_kernel_quantize_input(x, None, FP8, True),
+                  lambda x: flag_gems.moe_kernel_quantize_input(x, scale, FP8, False), lambda x: flag_gems.moe_kernel_quantize_input(x, None, FP8, False),
+                  lambda x: flag_gems.moe_kernel_quantize_input(x, None, FP8, False, [128, 64]), lambda x: flag_gems.per_token_group_quant_fp8(x, 64)]
+    x = _rand(3, 257, dtype=dtype)
+    for host in (_cabi.host, _Off()):
+        monkeypatch.setattr(_cabi, "host", host)
+        for quantise in quantisers:
+            want = quantise(x[:1, :256].clone(memory_format=torch.contiguous_format))
+            for got, w in zip(quantise(x[:1, :256]), want):
+                assert got.shape == w.shape and torch.equal(got.contiguous().view(torch.uint8), w.contiguous().view(torch.uint8))
