@@ -11,6 +11,7 @@ import os
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_uint, c_uint64, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libflaggems_b200.so")
@@ -219,6 +220,18 @@ def require_cuda(*tensors):
                 "flaggems_b200 runs on CUDA tensors only (sm_100a); got a tensor on "
                 f"{t.device}. There is no CPU path."
             )
+
+
+def has_tangent(t):
+    """Whether a tensor carries a forward-mode tangent that operators are to pass on."""
+    return torch._C._is_fwd_grad_enabled() and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None
+
+
+def refuse_gradients(**tensors):
+    """Raises for operands whose gradient or tangent the result would not carry."""
+    for name, t in tensors.items():
+        if t is not None and ((t.requires_grad and torch.is_grad_enabled()) or has_tangent(t)):
+            raise NotImplementedError(f"{name} has no gradient here: pass it detached, or call under torch.no_grad()")
 
 
 def device_status():

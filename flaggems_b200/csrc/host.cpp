@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -74,6 +75,14 @@ at::Tensor empty(at::IntArrayRef sizes, ScalarType dtype, const at::Tensor& like
 }
 
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// Whether a tensor carries a forward-mode tangent that operators are to pass on.
+bool has_tangent(const at::Tensor& t) {
+    return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
+}
+
+// Whether a result without a gradient would lose one of this operand (the Python code refuses it).
+bool loses_gradient(const at::Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || has_tangent(t); }
 
 // Rows of a tensor seen as [rows, last dimension]: true when one stride addresses them all.  A single row has any stride; it
 // counts as the row's length, which the kernels' checks of alignment take.
@@ -219,6 +228,7 @@ PyObject* token_quant_as(ScalarType to, PyObject* const* a, Py_ssize_t n) {
         int64_t m, k, ld;
         const at::Tensor* x = n == 1 ? cuda_tensor(a[0]) : nullptr;
         if (!x || dtype_code(x->scalar_type()) < 0 || !as_rows(*x, &m, &k, &ld)) return none();
+        if (to == ScalarType::Char && loses_gradient(*x)) return none();
         at::Tensor q, s;
         const int rc = unlocked([&] {
             c10::cuda::CUDAGuard guard(x->device());
@@ -383,6 +393,7 @@ PyObject* int8_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
         const at::Tensor *a = cuda_tensor(p[0]), *b = cuda_tensor(p[1]), *sa = cuda_tensor(p[2]), *sb = cuda_tensor(p[3]);
         if (!a || !b || !sa || !sb || a->scalar_type() != ScalarType::Char || b->scalar_type() != ScalarType::Char) return none();
         if (a->device() != b->device() || a->device() != sa->device() || a->device() != sb->device()) return none();
+        if (loses_gradient(*sa) || loses_gradient(*sb)) return none();
         if (!as_rows(*a, &m, &k, &ld) || ld % 16 || ld < k || (uintptr_t)a->data_ptr() % 16 || b->dim() != 2 || b->size(1) != k)
             return none();
         const int64_t cols = b->size(0);
@@ -399,7 +410,7 @@ PyObject* int8_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
         if (p[4] != Py_None) {
             bias = cuda_tensor(p[4]);
             if (!bias || dtype_code(bias->scalar_type()) < 0 || bias->dim() != 1 || bias->size(0) != cols || !bias->is_contiguous() ||
-                bias->device() != a->device())
+                bias->device() != a->device() || loses_gradient(*bias))
                 return none();
         }
         at::Tensor c;
@@ -427,6 +438,7 @@ PyObject* int8_grouped_mm(PyObject*, PyObject* const* p, Py_ssize_t n) {
         if (!a || !b || !sa || !sb || !offs || a->scalar_type() != ScalarType::Char || b->scalar_type() != ScalarType::Char) return none();
         for (const at::Tensor* t : {b, sa, sb, offs})
             if (t->device() != a->device()) return none();
+        if (loses_gradient(*sa) || loses_gradient(*sb)) return none();
         if (a->dim() != 2 || b->dim() != 3 || sb->dim() != 2 || offs->dim() != 1) return none();
         const int64_t m = a->size(0), k = a->size(1), groups = b->size(0), cols = b->size(1);
         if (m == 0 || cols == 0 || groups == 0 || k == 0 || k % 16 || b->size(2) != k || !b->is_contiguous()) return none();

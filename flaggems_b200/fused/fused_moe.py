@@ -101,7 +101,7 @@ def _int8_quantize(A, A_scale, per_act_token, block_shape=None):
     _cabi.require_cuda(A)
     if block_shape is not None or not per_act_token:
         raise NotImplementedError("int8 activations: only per-token quantisation is implemented")
-    return per_token_quant_int8(A)
+    return per_token_quant_int8(A.detach())  # without a gradient, as the FP8 forms
 
 
 def _group_quant(x, group, row_index=None, index_div=1, index_limit=0, n_rows_dev=None, out_rows=None):

@@ -19,6 +19,7 @@ def per_token_quant_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
     Returns ``(q, s)``: ``q`` int8 with the shape of ``x`` and ``s`` float32 of shape ``x.shape[:-1] + (1,)``.
     Rows have to start on 16-byte boundaries and K has to be a multiple of 8.
+    Has no gradient: an ``x`` that requires one is refused where it would be recorded.
     """
     logger.debug("GEMS PER TOKEN QUANT INT8")
     done = _cabi.host.token_quant_int8(x) if x.is_cuda else None
@@ -27,6 +28,7 @@ def per_token_quant_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     assert x.dim() >= 1, "x needs a last dimension"
     if x.dtype not in _cabi.DTYPE_CODE:
         raise NotImplementedError(f"unsupported dtype {x.dtype}")
+    _cabi.refuse_gradients(x=x)
     _cabi.require_cuda(x)
     k = x.shape[-1]
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)

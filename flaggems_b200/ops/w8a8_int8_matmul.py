@@ -56,7 +56,8 @@ def w8a8_int8_matmul(
 
     ``As`` float32: one value, or one per row ([...] or [..., 1]); ``Bs`` float32: one value, or one per
     output channel ([N] or [N, 1]); ``bias`` [N] in bf16, fp16 or fp32.  Returns [..., N] of ``output_dtype``
-    (bf16, fp16 or fp32).  The scales that ``per_token_quant_int8`` returns fit as they are.
+    (bf16, fp16 or fp32).  The scales that ``per_token_quant_int8`` returns fit as they are.  For inference: scales
+    and bias that require a gradient are refused where one would be recorded.
     """
     logger.debug("GEMS W8A8_INT8_MATMUL")
     if A.is_cuda:
@@ -67,6 +68,7 @@ def w8a8_int8_matmul(
     k = A.shape[-1]
     n = B.shape[0]
     _check_operands(A, B, k, B.shape[1], output_dtype)
+    _cabi.refuse_gradients(As=As, Bs=Bs, bias=bias)
     lead = tuple(A.shape[:-1])
     As = _scale(As, (lead, lead + (1,)), "As")
     Bs = _scale(Bs, ((n,), (n, 1)), "Bs")
@@ -108,6 +110,7 @@ def w8a8_int8_grouped_mm(
     ``As`` float32, one value per row ([M] or [M, 1]); ``Bs`` float32 [G, N]; ``offs`` int32 [G], ascending, read on the
     device; ``bias`` [N] or [G, N], added in fp32.  Returns [M, N] of ``output_dtype``; rows from offs[-1] on
     belong to no group and are zeros.  ``moe_permute`` returns rows and ``offs`` that fit, ``per_token_quant_int8`` scales.
+    For inference, as ``w8a8_int8_matmul``.
     """
     logger.debug("GEMS W8A8_INT8_GROUPED_MM")
     if A.is_cuda and bias is None:
@@ -118,6 +121,7 @@ def w8a8_int8_grouped_mm(
     m, k = A.shape
     g, n, k_b = B.shape
     _check_operands(A, B, k, k_b, output_dtype)
+    _cabi.refuse_gradients(As=As, Bs=Bs, bias=bias)
     assert tuple(As.shape) in ((m,), (m, 1)), f"As must have shape ({m},) or ({m}, 1)"
     assert tuple(Bs.shape) == (g, n), f"Bs must have shape ({g}, {n})"
     assert offs.shape == (g,) and offs.dtype == torch.int32, f"offs must be int32 of shape ({g},)"

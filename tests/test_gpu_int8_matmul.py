@@ -509,6 +509,30 @@ def test_native_and_python_host_paths_agree(monkeypatch):
         assert u.dtype == v.dtype and torch.equal(u, v)
 
 
+def test_gradients_that_would_be_lost_are_refused():
+    a, b, a_s, b_s, g = _operands(4, 96, 64)
+    ga, gb, ga_s, gb_s, offs, _ = _grouped([1, 0, 3], 96, 64)
+    bias, x = torch.randn(96, device="cuda", generator=g), torch.randn(4, 64, device="cuda", generator=g)
+    calls = [(lambda t: flag_gems.w8a8_int8_matmul(a, b, t, b_s), a_s), (lambda t: flag_gems.w8a8_int8_matmul(a, b, a_s, t), b_s),
+             (lambda t: flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, t), bias),
+             (lambda t: flag_gems.w8a8_int8_grouped_mm(ga, gb, t, gb_s, offs), ga_s),
+             (lambda t: flag_gems.w8a8_int8_grouped_mm(ga, gb, ga_s, t, offs), gb_s),
+             (lambda t: flag_gems.w8a8_int8_grouped_mm(ga, gb, ga_s, gb_s, offs, t), bias),
+             (lambda t: flag_gems.per_token_quant_int8(t)[0], x)]
+    for call, t in calls:
+        want, leaf = call(t), t.clone().requires_grad_()
+        with pytest.raises(NotImplementedError, match="has no gradient"):
+            call(leaf)
+        with torch.no_grad():
+            assert torch.equal(call(leaf), want)
+        assert torch.equal(call(leaf.detach()), want)
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="has no gradient"):
+                call(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+    q, s = flag_gems.moe_kernel_quantize_input(x.clone().requires_grad_(), None, I8, True)  # as its FP8 form: no gradient
+    assert torch.equal(q, flag_gems.per_token_quant_int8(x)[0]) and not s.requires_grad
+
+
 def test_another_stream_and_graph_capture():
     a, b, a_s, b_s, _ = _operands(16, 4096, 4096)
     ga, gb, ga_s, gb_s, offs, _ = _grouped([9, 0, 140], 96, 64)

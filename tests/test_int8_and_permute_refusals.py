@@ -1,6 +1,7 @@
 """Calls that w8a8_int8_matmul, w8a8_int8_grouped_mm, per_token_quant_int8, moe_permute and moe_unpermute refuse (no GPU)."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flag_gems
 from flaggems_b200 import _cabi
@@ -70,6 +71,29 @@ def test_matmul(over, error, text):
 def test_grouped(over, error, text):
     with pytest.raises(error, match=text):
         _grouped(**over)
+
+
+def _quant(x):
+    return flag_gems.per_token_quant_int8(x)
+
+
+GRADIENTS = [(_mm, "As", (3, 1)), (_mm, "Bs", (5,)), (_mm, "bias", (5,)), (_grouped, "As", (3,)), (_grouped, "Bs", (2, 5)),
+             (_grouped, "bias", (2, 5)), (_quant, "x", (2, 16))]
+
+
+@pytest.mark.parametrize("call,name,shape", GRADIENTS)
+def test_gradients_that_would_be_lost(call, name, shape):
+    t = torch.ones(shape, requires_grad=True)
+    with pytest.raises(NotImplementedError, match=f"{name} has no gradient"):
+        call(**{name: t})
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t.detach(), torch.ones(shape))
+        with pytest.raises(NotImplementedError, match=f"{name} has no gradient"), torch.no_grad():
+            call(**{name: dual})
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(_cabi.FlagGemsB200Error, match="CUDA tensors only"):
+            call(**{name: dual})
+    with torch.no_grad(), pytest.raises(_cabi.FlagGemsB200Error, match="CUDA tensors only"):
+        call(**{name: t})
 
 
 @pytest.mark.parametrize("over,error,text", [
