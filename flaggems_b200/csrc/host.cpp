@@ -663,6 +663,10 @@ void differentiable_once(torch::autograd::variable_list& grads, bool needed) {
     grads = (*error)(std::move(grads));
 }
 
+void refuse_tangents(const at::Tensor& gradient) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(gradient), "moe_permute and moe_unpermute have no forward-mode derivative");
+}
+
 at::Tensor unpermuted(const at::Tensor& rows, const at::Tensor& row_of_slot, const at::Tensor& weights) {
     c10::cuda::CUDAGuard guard(rows.device());
     const int64_t tokens = row_of_slot.size(0), hidden = rows.size(1);
@@ -721,6 +725,7 @@ struct PermuteFunction : torch::autograd::Function<PermuteFunction> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d) {
         torch::autograd::variable_list grads(6);
         if (!d[0].defined()) return grads;
+        refuse_tangents(d[0]);
         const bool again = d[0].requires_grad();
         {
             at::AutoDispatchBelowADInplaceOrView below;
@@ -744,6 +749,7 @@ struct UnpermuteFunction : torch::autograd::Function<UnpermuteFunction> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list d) {
         torch::autograd::variable_list grads(3);
         if (!d[0].defined()) return grads;
+        refuse_tangents(d[0]);
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &rows = saved[0], &row_of_slot = saved[1], &weights = saved[2];
         const bool w = weights.defined(), want_rows = ctx->needs_input_grad(0), want_w = w && ctx->needs_input_grad(2) && rows.defined();
@@ -781,13 +787,13 @@ PyObject* moe_permute(PyObject*, PyObject* const* p, Py_ssize_t n) {
             default: return none();
         }
         if (ids->scalar_type() != ScalarType::Int && ids->scalar_type() != ScalarType::Long) return none();
-        if (!ids->is_contiguous() || ids->size(0) != x->size(0) || ids->device() != x->device()) return none();
+        if (!ids->is_contiguous() || ids->size(0) != x->size(0) || ids->device() != x->device() || has_tangent(*x)) return none();
         const at::Tensor *scale = nullptr, *map = nullptr;
         const bool grad = at::GradMode::is_enabled();
         if (p[3] != Py_None) {
             scale = cuda_tensor(p[3]);
             if (!scale || scale->scalar_type() != ScalarType::Float || !rows_of_values(*scale) || scale->size(0) != x->size(0) ||
-                scale->device() != x->device() || (grad && scale->requires_grad()))
+                scale->device() != x->device() || loses_gradient(*scale))
                 return none();
         }
         if (p[4] != Py_None) {
@@ -825,13 +831,14 @@ PyObject* moe_unpermute(PyObject*, PyObject* const* p, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const at::Tensor *rows = n == 3 ? cuda_tensor(p[0]) : nullptr, *slots = rows ? cuda_tensor(p[1]) : nullptr;
         if (!slots || dtype_code(rows->scalar_type()) < 0 || !rows_of_values(*rows) || slots->scalar_type() != ScalarType::Int ||
-            slots->dim() != 2 || !slots->is_contiguous() || slots->device() != rows->device() || slots->numel() != rows->size(0))
+            slots->dim() != 2 || !slots->is_contiguous() || slots->device() != rows->device() || slots->numel() != rows->size(0) ||
+            has_tangent(*rows))
             return none();
         at::Tensor weights;
         if (p[2] != Py_None) {
             const at::Tensor* w = cuda_tensor(p[2]);
             if (!w || dtype_code(w->scalar_type()) < 0 || w->sizes() != slots->sizes() || !rows_of_values(*w) ||
-                w->device() != rows->device())
+                w->device() != rows->device() || has_tangent(*w))
                 return none();
             weights = *w;
         }

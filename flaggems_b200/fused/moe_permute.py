@@ -41,6 +41,11 @@ def _check_devices(first, *others):
         assert t is None or t.device == first.device, f"operands on {first.device} and {t.device}"
 
 
+def _refuse_tangents(*tensors):
+    if any(t is not None and _cabi.has_tangent(t) for t in tensors):
+        raise NotImplementedError("moe_permute and moe_unpermute have no forward-mode derivative")
+
+
 def _permute(x, topk_ids, num_experts, scale, expert_map):
     tokens, topk = topk_ids.shape
     hidden = x.shape[1]
@@ -86,6 +91,7 @@ class _Permute(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_rows, *_):
+        _refuse_tangents(d_rows)
         row_of_slot, = ctx.saved_tensors
         return _unpermute(_rows(d_rows, "the gradient"), row_of_slot, None), None, None, None, None
 
@@ -100,6 +106,7 @@ class _Unpermute(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
+        _refuse_tangents(d_out)
         rows, row_of_slot, weights = ctx.saved_tensors
         d_out = _rows(d_out, "the gradient")
         d_rows = d_weights = None
@@ -134,8 +141,9 @@ def moe_permute(
     zeros (their scales ones) and get no gradient back.
 
     Returns ``(rows [tokens * topk, hidden], row_scale or None, plan)``; ``plan.offs`` is what
-    ``w8a8_int8_grouped_mm`` and ``scaled_grouped_mm`` take.  Differentiable in ``hidden_states``, once.  A step that is
-    captured into a CUDA graph with its backward pass takes leaves of its own, as with every operator of torch.
+    ``w8a8_int8_grouped_mm`` and ``scaled_grouped_mm`` take.  Differentiable in ``hidden_states``, once and in
+    reverse mode.  A step that is captured into a CUDA graph with its backward pass takes leaves of its own, as with every
+    operator of torch.
     """
     logger.debug("GEMS MOE PERMUTE")
     if hidden_states.is_cuda:
@@ -157,6 +165,7 @@ def moe_permute(
         assert scale.shape[0] == x.shape[0], f"{x.shape[0]} tokens, {scale.shape[0]} rows of scales"
         if scale.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("scale has no gradient")
+    _refuse_tangents(x, scale)
     if expert_map is not None:
         assert expert_map.dim() == 1 and expert_map.numel() > 0, "expert_map must be 1-D and not empty"
         if expert_map.dtype not in (torch.int32, torch.int64):
@@ -181,7 +190,8 @@ def moe_unpermute(
 
     ``rows`` [tokens * topk, hidden] in bf16, fp16 or fp32; ``plan`` from ``moe_permute``; ``topk_weights``
     [tokens, topk] in bf16, fp16 or fp32, None for ones.  Slots without an expert add nothing and their rows are not
-    read.  Returns [tokens, hidden] of the type of ``rows``.  Differentiable in ``rows`` and ``topk_weights``, once.
+    read.  Returns [tokens, hidden] of the type of ``rows``.  Differentiable in ``rows`` and ``topk_weights``, once and in
+    reverse mode.
     """
     logger.debug("GEMS MOE UNPERMUTE")
     if rows.is_cuda:
@@ -199,6 +209,7 @@ def moe_unpermute(
         if topk_weights.dtype not in _cabi.DTYPE_CODE:
             raise NotImplementedError(f"unsupported dtype of topk_weights {topk_weights.dtype}")
         topk_weights = _rows(topk_weights, "topk_weights")
+    _refuse_tangents(rows, topk_weights)
     _check_devices(rows, row_of_slot, topk_weights)
     row_of_slot = row_of_slot.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (topk_weights is not None and topk_weights.requires_grad)):

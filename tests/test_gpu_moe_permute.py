@@ -6,6 +6,7 @@ type for the cast.
 """
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flag_gems
 from flaggems_b200 import _cabi
@@ -297,6 +298,39 @@ def test_no_gradient_without_asking():
     assert not rows.requires_grad and not out.requires_grad
     rows, _, plan = flag_gems.moe_permute(x, ids, 2)
     assert rows.requires_grad and not any(p.requires_grad for p in plan)
+
+
+class _Off:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_forward_mode_is_refused(native, monkeypatch):
+    """Tangents of the inputs, and of a gradient on its way back, are not dropped."""
+    if not native:
+        monkeypatch.setattr(_cabi, "host", _Off())
+    g = _gen(3)
+    t, k, e, h = 6, 2, 4, 16
+    ids, x, w = _ids(t, e, k, g), torch.randn(t, h, device="cuda", generator=g), torch.rand(t, k, device="cuda", generator=g)
+    rows, _, plan = flag_gems.moe_permute(x, ids, e)
+    out = flag_gems.moe_unpermute(rows, plan, w)
+    with forward_ad.dual_level():
+        def dual(v):
+            return forward_ad.make_dual(v, torch.ones_like(v))
+
+        for call in (lambda: flag_gems.moe_permute(dual(x), ids, e), lambda: flag_gems.moe_permute(dual(x.clone().requires_grad_()), ids, e),
+                     lambda: flag_gems.moe_permute(x, ids, e, scale=dual(w)), lambda: flag_gems.moe_unpermute(dual(rows), plan, w),
+                     lambda: flag_gems.moe_unpermute(rows, plan, dual(w)), lambda: flag_gems.moe_unpermute(dual(rows), plan)):
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                call()
+        x_, y_, w_ = (v.clone().requires_grad_() for v in (x, rows, w))
+        for result in (flag_gems.moe_permute(x_, ids, e)[0], flag_gems.moe_unpermute(y_, plan, w_), flag_gems.moe_unpermute(y_, plan)):
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                (result * dual(torch.ones_like(result))).sum().backward()
+        with forward_ad._set_fwd_grad_enabled(False):
+            assert torch.equal(flag_gems.moe_unpermute(dual(rows), plan, w), out)
+    assert torch.equal(flag_gems.moe_unpermute(rows, plan, w), out)
 
 
 def test_inf_and_nan_are_carried():

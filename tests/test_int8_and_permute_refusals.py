@@ -184,3 +184,11 @@ def test_entry_points_check_their_sizes():
 def test_expert_maps(expert_map, error, text):
     with pytest.raises(error, match=text):
         _permute(expert_map=expert_map)
+
+
+@pytest.mark.parametrize("call,name,shape", [(_permute, "hidden_states", (3, 16)), (_permute, "scale", (3, 1)), (_unpermute, "rows", (6, 16)),
+                                             (_unpermute, "topk_weights", (3, 2))])
+def test_forward_mode(call, name, shape):
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+            call(**{name: forward_ad.make_dual(torch.ones(shape), torch.ones(shape))})
