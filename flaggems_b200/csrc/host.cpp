@@ -789,7 +789,8 @@ PyObject* moe_permute(PyObject*, PyObject* const* p, Py_ssize_t n) {
         if (ids->scalar_type() != ScalarType::Int && ids->scalar_type() != ScalarType::Long) return none();
         if (!ids->is_contiguous() || ids->size(0) != x->size(0) || ids->device() != x->device() || has_tangent(*x)) return none();
         const at::Tensor *scale = nullptr, *map = nullptr;
-        const bool grad = at::GradMode::is_enabled();
+        const bool grad = at::GradMode::is_enabled() && x->requires_grad();
+        if (grad && dtype_code(x->scalar_type()) < 0) return none();  // gradients are summed in the types of moe_unpermute
         if (p[3] != Py_None) {
             scale = cuda_tensor(p[3]);
             if (!scale || scale->scalar_type() != ScalarType::Float || !rows_of_values(*scale) || scale->size(0) != x->size(0) ||
@@ -804,7 +805,7 @@ PyObject* moe_permute(PyObject*, PyObject* const* p, Py_ssize_t n) {
         }
         Permuted out;
         unlocked([&] {
-            if (grad && x->requires_grad()) {
+            if (grad) {
                 out.rows = PermuteFunction::apply(*x, *ids, experts, scale, map, &out);
             } else {
                 out = permuted(*x, *ids, experts, scale, map);

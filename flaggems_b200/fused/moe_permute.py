@@ -141,9 +141,9 @@ def moe_permute(
     zeros (their scales ones) and get no gradient back.
 
     Returns ``(rows [tokens * topk, hidden], row_scale or None, plan)``; ``plan.offs`` is what
-    ``w8a8_int8_grouped_mm`` and ``scaled_grouped_mm`` take.  Differentiable in ``hidden_states``, once and in
-    reverse mode.  A step that is captured into a CUDA graph with its backward pass takes leaves of its own, as with every
-    operator of torch.
+    ``w8a8_int8_grouped_mm`` and ``scaled_grouped_mm`` take.  Differentiable in ``hidden_states`` of
+    bf16, fp16 and fp32, once and in reverse mode.  A step that is captured into a CUDA graph with its backward pass takes
+    leaves of its own, as with every operator of torch.
     """
     logger.debug("GEMS MOE PERMUTE")
     if hidden_states.is_cuda:
@@ -155,6 +155,8 @@ def moe_permute(
         raise NotImplementedError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     if hidden_states.dtype not in _ELEMENT_BYTES:
         raise NotImplementedError(f"unsupported dtype {hidden_states.dtype}")
+    if hidden_states.dtype not in _cabi.DTYPE_CODE and hidden_states.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"hidden_states of {hidden_states.dtype} have no gradient")
     num_experts = int(num_experts)
     assert num_experts > 0, "num_experts must be positive"
     x = _rows(hidden_states, "hidden_states")

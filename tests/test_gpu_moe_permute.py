@@ -333,6 +333,17 @@ def test_forward_mode_is_refused(native, monkeypatch):
     assert torch.equal(flag_gems.moe_unpermute(rows, plan, w), out)
 
 
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2])
+def test_gradients_of_8_bit_floats_are_refused(dtype):
+    g = _gen(4)
+    ids, x = _ids(6, 4, 2, g), torch.randn(6, 16, device="cuda", generator=g).to(dtype)
+    with pytest.raises(NotImplementedError, match="have no gradient"):
+        flag_gems.moe_permute(x.clone().requires_grad_(), ids, 4)
+    with torch.no_grad():
+        rows, _, plan = flag_gems.moe_permute(x.clone().requires_grad_(), ids, 4)
+    _check_permuted(x, rows, plan, 2)
+
+
 def test_inf_and_nan_are_carried():
     x = torch.tensor([[1.0, float("inf")], [float("nan"), -0.0], [3.0, 65504.0]], device="cuda")
     ids = torch.tensor([[1, 0], [0, -1], [1, 1]], dtype=torch.int32, device="cuda")

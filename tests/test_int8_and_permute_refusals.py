@@ -192,3 +192,12 @@ def test_forward_mode(call, name, shape):
     with forward_ad.dual_level():
         with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
             call(**{name: forward_ad.make_dual(torch.ones(shape), torch.ones(shape))})
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2])
+def test_gradients_of_8_bit_floats(dtype):
+    x = torch.zeros(3, 16).to(dtype).requires_grad_()
+    with pytest.raises(NotImplementedError, match="have no gradient"):
+        _permute(hidden_states=x)
+    with torch.no_grad(), pytest.raises(_cabi.FlagGemsB200Error, match="CUDA tensors only"):
+        _permute(hidden_states=x)
