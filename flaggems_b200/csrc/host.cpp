@@ -165,6 +165,8 @@ PyObject* guarded(F&& f) {
         PyErr_SetString(cls ? cls : PyExc_MemoryError, e.what_without_backtrace());
         Py_XDECREF(cls);
         Py_XDECREF(torch_mod);
+    } catch (const c10::NotImplementedError& e) {
+        PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     }

@@ -344,6 +344,15 @@ def test_gradients_of_8_bit_floats_are_refused(dtype):
     _check_permuted(x, rows, plan, 2)
 
 
+@pytest.mark.parametrize("native", [True, False])
+def test_rows_too_long_are_refused_alike(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_cabi, "host", _Off())
+    x, ids = torch.empty(1, 1 << 31, dtype=torch.int8, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(NotImplementedError, match="size too large"):
+        flag_gems.moe_permute(x, ids, 1)
+
+
 def test_inf_and_nan_are_carried():
     x = torch.tensor([[1.0, float("inf")], [float("nan"), -0.0], [3.0, 65504.0]], device="cuda")
     ids = torch.tensor([[1, 0], [0, -1], [1, 1]], dtype=torch.int32, device="cuda")
