@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(ALIGN_THREADS, 1) group_tiles_kernel(const int
     int32_t lo = 0, count = 0;
     if (g < num_groups) {
         lo = g > 0 ? min(max(offs[g - 1], 0), rows) : 0;
-        count = max(min(offs[g], rows) - lo, 0);
+        count = max(min(max(offs[g], 0), rows) - lo, 0);
     }
     const int32_t padded = (count + block - 1) / block * block;
     int32_t incl = padded;

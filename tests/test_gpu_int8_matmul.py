@@ -361,6 +361,20 @@ def test_grouped_few_rows_of_ends_out_of_range():
     assert _cabi.device_status() == 0
 
 
+def test_grouped_ends_out_of_range():
+    """As above for more rows, whose tables of tiles a kernel of their own makes."""
+    a, b, a_s, b_s, offs, _ = _grouped([20, 0, 30, 10], 515, 272, tail=3)
+    want = _grouped_definition(a, b, a_s, b_s, offs)
+    low, high = torch.iinfo(torch.int32).min, torch.iinfo(torch.int32).max
+    ends = torch.tensor([20, low, 50, 60], dtype=torch.int32, device="cuda")  # groups 0 and 2 share the first 20 rows
+    got = flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, ends, output_dtype=torch.float32)
+    _check(got[20:], want[20:])
+    ends = torch.tensor([20, 20, 50, high], dtype=torch.int32, device="cuda")  # the last group takes what is left
+    want[50:] = _definition(a[50:], b[3], a_s[50:], b_s[3])
+    _check(flag_gems.w8a8_int8_grouped_mm(a, b, a_s, b_s, ends, output_dtype=torch.float32), want)
+    assert _cabi.device_status() == 0
+
+
 def test_grouped_ends_that_the_kernel_before_writes():
     a, b, a_s, b_s, offs, g = _grouped([4] * 4, 4096, 1024)
     kept = []
