@@ -99,7 +99,8 @@ bool fg_int8_is_skinny_grouped(int64_t M, int64_t N, int n_experts);
 int fg_int8_skinny_grouped(const FgSkinny& p, const int32_t* offs, int n_experts, int64_t bias_stride, cudaStream_t st);
 
 // Tile of an int8 product: its width and kind (one CTA per 128 rows, or a CTA pair per 256) with the least estimated
-// time, for so many blocks of rows of either kind (blocks256 0: no pairs) and tiles of at least `narrowest` columns.
+// time, for so many blocks of rows of either kind (blocks256 0: no pairs) and tiles of at least `narrowest` columns (64; 96 for
+// grouped products, which are not built 64 wide).
 struct FgInt8Tile {
     bool pair;
     int width;

@@ -1805,7 +1805,7 @@ FgInt8Tile fg_int8_tile(int64_t blocks128, int64_t blocks256, int64_t N, int64_t
             best = FgInt8Tile{pair, width, time};
         }
     };
-    for (int width = 256; width >= 96; width -= 32) offer(false, width, 4000, 290 + 130 * width / 256);
+    for (int width = 256; width >= 96 && width >= narrowest; width -= 32) offer(false, width, 4000, 290 + 130 * width / 256);
     if (narrowest <= 64) offer(false, 64, 4000, 285);
     if (blocks256 > 0 && pair_enabled())
         for (int width = 256; width >= 128; width -= 32) offer(true, width, 5500, 265 + 80 * width / 256);

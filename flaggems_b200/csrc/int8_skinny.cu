@@ -571,7 +571,7 @@ int launch(StreamArgs& a, cudaStream_t st) {
     return FG_OK;
 }
 
-// Stages of 20 to 48 KB: the lower a group, the more blocks of K.
+// Stages of 19 to 48 KB (64 with 17 to 32 tokens and 32 rows): the lower a group, the more blocks of K.
 template <bool GROUPED>
 int launch_registers(StreamArgs& a, cudaStream_t st) {
     auto by_rows = [&](auto nt) -> int {

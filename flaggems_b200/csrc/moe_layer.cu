@@ -264,7 +264,7 @@ int scaled_grouped_mm(int operand, void* c, const void* a, const void* b, const 
     const bool few_waves = m_total >= 96 * (int64_t)num_groups && blocks * fg_cdiv(N, 256) <= 4 * (int64_t)fg_num_sms();
     if (operand == 1 && (few_waves || m_total >= 448 * (int64_t)num_groups)) {
         const bool enough = m_total >= INT8_PAIR_MIN_ROWS * (int64_t)num_groups;
-        const FgInt8Tile t = fg_int8_tile(blocks, enough ? m_total / PAIR_ROWS + (num_groups + 1) / 2 : 0, N, K, 128);
+        const FgInt8Tile t = fg_int8_tile(blocks, enough ? m_total / PAIR_ROWS + (num_groups + 1) / 2 : 0, N, K, 96);
         pairs = t.pair;
         width = t.width;
     }
