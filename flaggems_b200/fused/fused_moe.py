@@ -77,25 +77,6 @@ def _per_token_quant(x, row_index=None, index_div=1, index_limit=0, n_rows_dev=N
     return q, s
 
 
-def _per_token_quant_int8(x, row_index=None, index_div=1, index_limit=0, n_rows_dev=None, out_rows=None):
-    """Dynamic per-row INT8 quantisation (reference: fused_moe.py:732-739), optionally gathering rows
-    through ``row_index``."""
-    k = x.shape[-1]
-    x2 = x.reshape(-1, k)
-    rows = x2.shape[0] if out_rows is None else out_rows
-    q = torch.empty((rows, k), dtype=torch.int8, device=x.device)
-    s = torch.empty((rows, 1), dtype=torch.float32, device=x.device)
-    if rows and k:
-        _cabi.check(
-            _cabi.lib().fg_per_token_quant_int8(
-                _cabi.ptr(x2), _cabi.DTYPE_CODE[x.dtype], _cabi.ptr(q), _cabi.ptr(s), rows, k,
-                _cabi.row_stride(x2), k, _cabi.ptr(row_index), index_div, index_limit, _cabi.ptr(n_rows_dev),
-                _cabi.stream_ptr(x.device),
-            )
-        )
-    return q, s
-
-
 def _int8_quantize(A, A_scale, per_act_token, block_shape=None):
     """INT8 quantisation of MoE activations (reference: fused_moe.py:700-747); the per-token form only."""
     _cabi.require_cuda(A)
