@@ -1368,11 +1368,12 @@ int launch_splitk(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams
     return FG_OK;
 }
 
-// int8 products with few tiles and a long K: the width of a tile and the slices of K (a cluster's CTAs, one wave of them) with the least
-// estimated time, if that is below 95 % of `least` ns, the time of a form without; slices 1 otherwise.  A block of K costs what it
-// does in fg_int8_tile; the rest is the launch of clusters and the sum over their shared memory.  Measured, without / split: 129 x
-// 1000 x 8192 22.1 / 12.3 us (64 wide, 4 slices), 129 x 4096 x 14336 37.4 / 28.3 (128, 2), 128 x 4096 x 14336 24.2 / 20.8 (128, 4),
-// 256 x 2112 x 7168 19.9 / 16.5 (128, 3); 129 x 4096 x 4096 13.6 / 14.8, which stays whole.
+// int8 products (from 17 rows on) with few tiles and a long K: the width of a tile and the slices of K (a cluster's CTAs, one
+// wave of them) with the least estimated time, if that is below 95 % of `least` ns, the time of a form without; slices 1
+// otherwise.  A block of K costs what it does in fg_int8_tile; the rest is the launch of clusters and the sum over their
+// shared memory.  Measured, without / split: 129 x 1000 x 8192 22.1 / 12.3 us (64 wide, 4 slices), 129 x 4096 x 14336 37.4 / 28.3
+// (128, 2), 128 x 4096 x 14336 24.2 / 20.8 (128, 4), 256 x 2112 x 7168 19.9 / 16.5 (128, 3); 129 x 4096 x 4096 13.6 / 14.8,
+// which stays whole.
 struct Int8Split {
     int width, slices;
 };

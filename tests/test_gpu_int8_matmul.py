@@ -133,6 +133,20 @@ def test_long_rows_and_narrow_weights(m, n, k, out, bias):
     assert _cabi.device_status() == 0
 
 
+# rows below 65: fewer than 128 of them in shared memory, and CTAs of the cluster whose share of the rows is small or empty
+@pytest.mark.parametrize("m,n,k", [(33, 16, 65536), (33, 100, 32768), (40, 1000, 16384), (64, 130, 32768), (64, 4096, 16384), (57, 33, 131056),
+                                   (20, 6000, 32768), (31, 5001, 32784)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("bias", [None, torch.float32])
+def test_few_rows_with_split_k(m, n, k, out, bias):
+    a, b, a_s, b_s, g = _operands(m, n, k, seed=m)
+    c = None if bias is None else torch.randn(n, device="cuda", generator=g).to(bias)
+    got = flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, c, out)
+    _check(got, _definition(a, b, a_s, b_s), c)
+    assert torch.equal(got, flag_gems.w8a8_int8_matmul(a, b, a_s, b_s, c, out))
+    assert _cabi.device_status() == 0
+
+
 @pytest.mark.parametrize("m,n,k", [(128, 1000, 8192), (300, 576, 7168)])
 def test_split_products_in_streams_and_graphs(m, n, k):
     """Operands that the kernel before writes, two streams at once, and two captured graphs replayed with other operands."""
