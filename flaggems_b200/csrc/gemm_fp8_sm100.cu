@@ -1789,10 +1789,11 @@ int fg_grouped_gemm_fp8_bias(void* c, const void* a, const void* w, const float*
 // The estimate is the number of waves of tiles times what a block of K takes, which hardly depends on the width below 256
 // (the ring's round trip; above, the 64 bytes per cycle that an SM takes in).  So a narrower tile pays where it saves a
 // wave, and a pair where a tile's K is long enough for its dearer start.  The constants (ns) are fitted to 5 weights x 12 row
-// counts x 11 tiles; the choices are within 6 % of the best of the 11.  Measured, 256-wide single / 256-wide pair / this:
-// 1037 x 6144 x 4096 32.3 / 28.7 / 27.0 us (pairs of 224 columns, two full waves), 300 x 7168 x 2048 13.3 / 13.2 / 12.0
-// (single, 160), 777 x 4096 x 14336 51.1 / 44.1 / 44.1, 1037 x 4096 x 14336 52.3 / 75.0 / 52.3, 256 x 6144 x 4096 19.6 /
-// 17.5 / 15.4 (single, 96).
+// counts x 11 tiles; the choices are within 6 % of the best of the 11.  Measured, 256-wide single / 256-wide pair / this, in a
+// stream with bf16 results: 1037 x 6144 x 4096 31.3 / 28.9 / 27.6 us (pairs of 224 columns, two full waves; 29.4 to 30.8 in fp16
+// with bias), 300 x 7168 x 2048 13.3 / 13.5 / 11.9 (single, 160), 777 x 4096 x 14336 53.1 / 48.4 / 48.3, 1037 x 4096 x
+// 14336 59.7 / 74.8 / 59.2, 256 x 6144 x 4096 19.6 / 17.1 / 16.3 (single, 96).  The weight's stream from HBM is not in it: where that
+// counts it is off by 7 % (scaled_grouped_mm).
 FgInt8Tile fg_int8_tile(int64_t blocks128, int64_t blocks256, int64_t N, int64_t K, int narrowest) {
     const int sms = fg_num_sms();
     const int64_t k_blocks = fg_cdiv(K, BLOCK_K);

@@ -11,8 +11,9 @@
 //   up to 128         one thread with tcgen05 (kind::i8), tokens as M and weight rows as N, into TMEM.
 //
 // Against the tiles that serve more tokens (128 x 256 and the like, with K split over a cluster) this saves the padding to 128
-// rows, the SMs that 256-row tiles leave without one, and the reduction: 1 x 6144 x 4096 6.3 us (11.0), 16 x 28672 x 4096 22.7
-// (26.6), 64 x 6144 x 4096 9.0 (15.9), 128 x 2112 x 7168 12.8 (17.6), 128 x 7168 x 2048 7.1 (18.7).
+// rows, the SMs that 256-row tiles leave without one, and the reduction: 1 x 6144 x 4096 6.8 us (11.0), 16 x 28672 x 4096 21.7
+// (26.6), 64 x 6144 x 4096 9.1 (15.9), 128 x 2112 x 7168 12.9 (17.6), 128 x 7168 x 2048 7.3 (18.7); bf16 results, in a stream,
+// inputs rotated through more than L2 (the first takes 5.3 to 6.4 where two to four weights take turns).
 //
 // K is a sum, so its order is free: with mma.m16n8k32, lane (g, t) of a warp takes bytes [32 t, 32 t + 32) of a block's rows,
 // for the weight and the tokens alike, as two 16-byte loads without bank conflicts, not the 4-byte pieces that the

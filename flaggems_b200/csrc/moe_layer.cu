@@ -257,9 +257,9 @@ int scaled_grouped_mm(int operand, void* c, const void* a, const void* b, const 
     bool pairs = use_pairs(m_total, num_groups, N, N);
     int width = 0;
     // int8: by the estimate for tiles, where the rows of a group make up for its weight or a few waves of tiles are all there
-    // is.  In between the weights' stream decides, and the plain rule does better.  Estimate / plain rule, 8 groups: 2048 x
-    // 4096 x 14336 161 / 184 us, 6000 x 4096 x 14336 277 / 306, 6000 x 28672 x 4096 538 / 599; but 2048 x 28672 x 4096 302 / 271,
-    // and 1536 x 4096 x 7168 in 32 groups 175 / 163.
+    // is.  In between the weights' stream decides, and the plain rule does better.  Estimate / plain rule, bf16 results, 8 groups of
+    // random rows: 2048 x 4096 x 14336 171 / 175 us, 6000 x 4096 x 14336 342 / 363, 6000 x 28672 x 4096 657 / 698; but 2048 x 28672 x
+    // 4096 338 / 318, and 1536 x 4096 x 7168 in 32 groups 193 / 185.
     const int64_t blocks = m_total / TILE_ROWS + (num_groups + 1) / 2;  // a group ends half a block before its last block, on average
     const bool few_waves = m_total >= 96 * (int64_t)num_groups && blocks * fg_cdiv(N, 256) <= 4 * (int64_t)fg_num_sms();
     if (operand == 1 && (few_waves || m_total >= 448 * (int64_t)num_groups)) {
